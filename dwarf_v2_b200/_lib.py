@@ -296,9 +296,35 @@ class LseReduceArgs(ctypes.Structure):
         target_logit:ptr, ignore_index:i64, lse:ptr, argmax:ptr, loss:ptr""")
 
 
+class TokenLogprobsArgs(ctypes.Structure):
+    _fields_ = _fields("""version:i32, dtype:i32, logits:ptr, outer:i64, inner:i64, vocab:i64, so:i64, si:i64,
+        targets:ptr, ignore_index:i64, inv_temperature:f32, top_k:i32, logprob:ptr, entropy:ptr, lse:ptr, stats:ptr,
+        top_logprobs:ptr, top_ids:ptr""")
+
+
+class TokenLogprobsBwdArgs(ctypes.Structure):
+    _fields_ = _fields("""version:i32, dtype:i32, logits:ptr, outer:i64, inner:i64, vocab:i64, so:i64, si:i64,
+        targets:ptr, ignore_index:i64, inv_temperature:f32, top_k:i32, stats:ptr, entropy:ptr, top_ids:ptr,
+        g_logprob:ptr, g_entropy:ptr, g_lse:ptr, g_top:ptr, grad:ptr""")
+
+
+class TopkDistillArgs(ctypes.Structure):
+    _fields_ = _fields("""version:i32, dtype:i32, logits:ptr, outer:i64, inner:i64, vocab:i64, so:i64, si:i64,
+        teacher_ids:ptr, teacher_logprobs:ptr, k:i32, tail:i32, row_mask:ptr, inv_temperature:f32,
+        grad_rows_stride:i32, grad_scale:ptr, grad_rows:ptr, loss:ptr, grad:ptr, skip_if_one:i32, loss_scale:f32, scale:f32""")
+
+
+class RowReduceArgs(ctypes.Structure):
+    _fields_ = _fields("""version:i32, rows:i64, values:ptr, mask:ptr, scale:ptr, host_scale:f32, out:ptr""")
+
+
 _ENTRY_POINTS = {
     "dwarf_gemm_bf16": GemmArgs,
     "dwarf_lse_reduce": LseReduceArgs,
+    "dwarf_token_logprobs": TokenLogprobsArgs,
+    "dwarf_token_logprobs_bwd": TokenLogprobsBwdArgs,
+    "dwarf_topk_distill": TopkDistillArgs,
+    "dwarf_row_reduce": RowReduceArgs,
     "dwarf_hisa_reps": HisaRepsArgs,
     "dwarf_hisa_select": HisaSelectArgs,
     "dwarf_hisa_attn": HisaAttnArgs,

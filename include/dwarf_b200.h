@@ -726,6 +726,134 @@ typedef struct {
 
 int dwarf_lse_reduce(const dwarf_lse_reduce_args* args, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Vocabulary rows: log probabilities of given tokens with the entropy and the
+ * best alternatives, and distillation from a teacher's top entries. Both read
+ * logits [outer, inner, vocab] (rows = outer * inner, row r = (r / inner,
+ * r % inner), unit stride on vocab, any row strides: logits[:, :-1] is read in
+ * place) of dtype DWARF_F32, DWARF_BF16 or DWARF_F16, vocab <= 2^20, and work
+ * on x / temperature. All sums and softmax statistics are fp32.
+ *
+ * dwarf_token_logprobs, per row, with c = 1/temperature, m = max x, S = sum
+ * exp(c (x - m)):
+ *   lse      = c m + log S
+ *   logprob  = c x[target] - lse; 0 where target == ignore_index, NaN for any
+ *              other target outside [0, vocab)
+ *   entropy  = log S - sum exp(c (x - m)) c (x - m) / S
+ *   top_ids / top_logprobs: the top_k largest logits, ties to the lowest id
+ * It stands beside dwarf_gemm_bf16's epilogue 4 (lse / argmax / loss of the
+ * lm_head) for logits that exist (a decoding step's, a trainer's).
+ * A row without a finite logit (all -inf): lse, logprob and top_logprobs -inf,
+ * entropy 0, top_ids 0..top_k-1. A row with NaN or +inf: every float NaN, the
+ * ids those of the order -inf < finite < +inf < NaN.
+ * ---------------------------------------------------------------------- */
+#define DWARF_TOP_K_MAX 128
+#define DWARF_VOCAB_MAX (1 << 20)
+
+typedef struct {
+  int32_t version;
+  int32_t dtype;                  /* of logits                             */
+  const void* logits;             /* [outer, inner, vocab]                 */
+  int64_t outer, inner, vocab;
+  int64_t so, si;                 /* row strides of logits                 */
+  const int64_t* targets;         /* optional [rows]                       */
+  int64_t ignore_index;
+  float inv_temperature;          /* finite, > 0                           */
+  int32_t top_k;                  /* 0..min(DWARF_TOP_K_MAX, vocab)        */
+  float* logprob;                 /* [rows] (with targets)                 */
+  float* entropy;                 /* [rows]                                */
+  float* lse;                     /* [rows]                                */
+  float* stats;                   /* optional float2 [rows]: (m, S), what
+                                     dwarf_token_logprobs_bwd reads        */
+  float* top_logprobs;            /* [rows, top_k]                         */
+  int64_t* top_ids;               /* [rows, top_k]                         */
+} dwarf_token_logprobs_args;
+
+int dwarf_token_logprobs(const dwarf_token_logprobs_args* args, void* stream);
+
+/* Gradient of the logits (in their dtype, rounded once) from the gradients of
+ * logprob, entropy, lse and top_logprobs (each optional):
+ *   G = g_logprob + sum_k g_top_k - g_lse,  q = exp(c x - lse)
+ *   grad_v = c (sum over entries with id v of their g - q_v (G + g_entropy (log q_v + entropy)))
+ * A row whose gradients are all zero, or without a finite logit, gets exact
+ * zeros and its logits are not used; a row whose target is neither
+ * ignore_index nor in [0, vocab) gets NaN when g_logprob is given. */
+typedef struct {
+  int32_t version;
+  int32_t dtype;                  /* of logits and grad                    */
+  const void* logits;             /* [outer, inner, vocab]                 */
+  int64_t outer, inner, vocab;
+  int64_t so, si;
+  const int64_t* targets;         /* as in the forward                     */
+  int64_t ignore_index;
+  float inv_temperature;
+  int32_t top_k;
+  const float* stats;             /* of the forward                        */
+  const float* entropy;           /* of the forward                        */
+  const int64_t* top_ids;         /* of the forward                        */
+  const float* g_logprob;         /* optional [rows]                       */
+  const float* g_entropy;         /* optional [rows]                       */
+  const float* g_lse;             /* optional [rows]                       */
+  const float* g_top;             /* optional [rows, top_k]                */
+  void* grad;                     /* [rows, vocab], contiguous             */
+} dwarf_token_logprobs_bwd_args;
+
+int dwarf_token_logprobs_bwd(const dwarf_token_logprobs_bwd_args* args, void* stream);
+
+/* Divergence KL(teacher || student) per row from the teacher's log
+ * probabilities of k listed ids, and its gradient, in one pass over the
+ * student's logits:
+ *   tail = 1: p_k = exp(l_k), p_* = max(0, 1 - sum p_k) for the ids not listed
+ *   tail = 0: p = softmax of the k values, no rest
+ *   loss = sum_k p_k (log p_k - log q_k) + p_* (log p_* - log q_*)
+ * with q = softmax(x / temperature) and q_* its sum over the ids not listed
+ * (p_* = 0 when every id is listed). Slots with an id below 0 are not used; an
+ * id >= vocab makes its row NaN; an id listed twice counts with both p. Rows
+ * with row_mask 0 or without a used slot: loss and gradient exact zeros, the
+ * logits not used.
+ *   grad_v = s c (q_v (sum p + p_*) - sum over slots with id v of p - [v not listed] p_* q_v / q_*)
+ * where s = scale * (grad_scale ? *grad_scale : 1) * (grad_rows ? grad_rows[row or 0] : 1).
+ * With skip_if_one the launch leaves grad as it is when grad_rows[0] == 1 (the
+ * gradient that the forward launch has written stands). */
+typedef struct {
+  int32_t version;
+  int32_t dtype;                  /* of logits and grad                    */
+  const void* logits;             /* [outer, inner, vocab]                 */
+  int64_t outer, inner, vocab;
+  int64_t so, si;
+  const int64_t* teacher_ids;     /* [rows, k], contiguous                 */
+  const float* teacher_logprobs;  /* [rows, k], contiguous                 */
+  int32_t k;                      /* 1..DWARF_TOP_K_MAX                    */
+  int32_t tail;                   /* 0 or 1                                */
+  const uint8_t* row_mask;        /* optional [rows]: 0 or 1               */
+  float inv_temperature;
+  int32_t grad_rows_stride;       /* 0: one scalar, 1: one per row         */
+  const float* grad_scale;        /* optional device scalar                */
+  const float* grad_rows;         /* optional device scalar or [rows]      */
+  float* loss;                    /* optional [rows]                       */
+  void* grad;                     /* optional [rows, vocab], contiguous    */
+  int32_t skip_if_one;            /* with grad_rows, stride 0, no loss     */
+  float loss_scale;               /* factor of loss                        */
+  float scale;                    /* factor of grad                        */
+} dwarf_topk_distill_args;
+
+int dwarf_topk_distill(const dwarf_topk_distill_args* args, void* stream);
+
+/* One fp32 value from rows: with `values`, out = (scale ? *scale : 1) * sum of
+ * values in a fixed order; without, out = 1 / max(1, number of mask bytes set),
+ * the scale of a mean over the rows that count. */
+typedef struct {
+  int32_t version;
+  int64_t rows;
+  const float* values;            /* optional [rows]                       */
+  const uint8_t* mask;            /* [rows] (without values)               */
+  const float* scale;             /* optional device scalar                */
+  float host_scale;               /* a further factor                      */
+  float* out;                     /* [1]                                   */
+} dwarf_row_reduce_args;
+
+int dwarf_row_reduce(const dwarf_row_reduce_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

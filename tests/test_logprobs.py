@@ -1,0 +1,466 @@
+"""Token log probabilities, entropy and top alternatives of logit rows, and their gradient,
+against the 64-bit oracle (oracle/vocab.py).
+
+Tolerances. One exponential is off by at most 2^-22 (ex2.approx) plus the rounding of its
+exponent d = c (x - m) log2 e (three roundings of 2^-24 relative: |d| ln2 3 2^-24). A sum over V
+entries adds at most N 2^-24 where N is the number of additions that one value passes: under
+V / 128 + 64 in any split of a row over threads. So a sum of exponentials is off by
+``rel = 2^-21 + (V / 128 + 64) 2^-24`` at the weight e (1 + |d|) <= 1 of its terms, a logarithm of it by
+the same absolute amount, and lse, logprob by that and two roundings (2^-23) of their own size and of the
+row maximum's. The entropy is a quotient of two such sums: rel (2 + entropy).
+Gradients are held entry by entry to rel times the sum of the magnitudes of their terms, with |d| ln2 2^-22
+for the exponent, plus the one rounding of the type (eps / 2 of the value; the smallest subnormal of fp16).
+"""
+
+import math
+
+import pytest
+import torch
+
+from oracle import vocab as oracle
+
+TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def rel_of(V):
+    return 2.0 ** -21 + (V / 128 + 64) * 2.0 ** -24
+
+
+def close(got, want, tol, what=""):
+    got, want = got.double().cpu(), want.double().cpu()
+    tol = torch.as_tensor(tol, dtype=torch.float64).cpu().expand(want.shape)
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    assert torch.equal(got[~fine & ~torch.isnan(want)], want[~fine & ~torch.isnan(want)]), what
+    off = (got - want).abs()[fine] - tol[fine]
+    assert off.numel() == 0 or off.max() <= 0, (what, float(off.max()), float((got - want).abs()[fine].max()))
+
+
+def check_forward(out, x, targets, k, t, ignore_index=-100):
+    R, V = x.numel() // x.shape[-1], x.shape[-1]
+    want = oracle.token_logprobs(x.reshape(R, V), None if targets is None else targets.reshape(R), top_k=k,
+                                 temperature=t, ignore_index=ignore_index)
+    rel = rel_of(V)
+    # a row without a finite logit has a maximum of 0 here: its outputs are exact values
+    top = torch.nan_to_num(x.double().reshape(R, V).amax(-1) / t, nan=0.0, posinf=0.0, neginf=0.0).abs()
+
+    def tol(v):
+        return rel + 2.0 ** -22 * torch.nan_to_num(want[v], nan=0.0, posinf=0.0, neginf=0.0).abs()
+
+    close(out.lse.reshape(R), want["lse"], tol("lse") + 2.0 ** -23 * top, "lse")
+    h = torch.nan_to_num(want["entropy"], nan=0.0)
+    close(out.entropy.reshape(R), want["entropy"], rel * (2.0 + 2.0 * h + math.log(V)), "entropy")
+    if targets is None:
+        assert out.logprob is None
+    else:
+        close(out.logprob.reshape(R), want["logprob"], tol("logprob"), "logprob")
+    if k:
+        assert torch.equal(out.top_ids.reshape(R, k).cpu(), want["top_ids"].cpu())
+        close(out.top_logprobs.reshape(R, k), want["top_logprobs"], tol("top_logprobs"), "top_logprobs")
+    else:
+        assert out.top_ids is None and out.top_logprobs is None
+    return want
+
+
+def grad_tolerance(x, t, grad, size):
+    V = x.shape[-1]
+    d = torch.nan_to_num((x.double() - x.double().amax(-1, keepdim=True)) / t, neginf=0.0).abs()
+    tiny = 2.0 ** -24 if x.dtype == torch.float16 else 2.0 ** -120
+    return size * (4 * rel_of(V) + d * 2.0 ** -21) + torch.finfo(x.dtype).eps / 2 * grad.abs() * 1.01 + tiny
+
+
+def logits(R, V, dtype, seed, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(R, V, generator=g) * spread).to(TYPES[dtype])
+
+
+# ------------------------------------------------------------------ CPU: the oracle, refusals
+
+
+def test_oracle_gradient_against_differences():
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(3, 11, generator=g, dtype=torch.float64)
+    targets = torch.tensor([4, -100, 0])
+    gl, gh, gz = (torch.randn(3, generator=g, dtype=torch.float64) for _ in range(3))
+    gt = torch.randn(3, 2, generator=g, dtype=torch.float64)
+    out = oracle.token_logprobs(x, targets, top_k=2, temperature=1.7)
+
+    def value(v):
+        o = oracle.token_logprobs(v, targets, temperature=1.7)
+        logq = v / 1.7 - o["lse"].unsqueeze(-1)
+        return ((gl * o["logprob"] + gh * o["entropy"] + gz * o["lse"]).sum()
+                + (gt * logq.gather(-1, out["top_ids"])).sum())
+
+    grad, _ = oracle.token_logprobs_grad(x, targets, top_ids=out["top_ids"], g_logprob=gl, g_entropy=gh, g_lse=gz,
+                                         g_top=gt, temperature=1.7)
+    for i in range(3):
+        for v in range(11):
+            step = torch.zeros_like(x)
+            step[i, v] = 1e-5
+            diff = (value(x + step) - value(x - step)) / 2e-5
+            assert abs(diff - grad[i, v]) < 1e-8
+
+
+def test_refuses_what_it_does_not_take():
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    x = torch.zeros(4, 10)
+    with pytest.raises(RuntimeError):
+        token_logprobs(x)
+    with pytest.raises(TypeError):
+        token_logprobs(x.double())
+    with pytest.raises(TypeError):
+        token_logprobs(x, torch.zeros(4))
+    for bad in (-1, 11, 129):
+        with pytest.raises(ValueError):
+            token_logprobs(x, top_k=bad)
+    with pytest.raises(ValueError):
+        token_logprobs(torch.zeros(4, 300), top_k=129)
+    for bad in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError):
+            token_logprobs(x, temperature=bad)
+    with pytest.raises(ValueError):
+        token_logprobs(x, torch.zeros(5, dtype=torch.int64))
+    with pytest.raises(ValueError):
+        token_logprobs(torch.zeros(4, 0))
+    with pytest.raises(ValueError):
+        token_logprobs(torch.zeros(()))
+    with pytest.raises(ValueError):
+        token_logprobs(torch.zeros(1, (1 << 20) + 1))
+
+
+def test_row_addressing():
+    from dwarf_v2_b200._rows import addressed
+
+    x = torch.zeros(4, 6, 10)
+    assert addressed(x)[1:] == (1, 24, 0, 10)
+    assert addressed(x[:, :-1])[1:] == (4, 5, 60, 10)
+    assert addressed(x[:, -1])[1:] == (1, 4, 0, 60)
+    assert addressed(x[0, 0])[1:] == (1, 1, 0, 0)
+    assert addressed(x[:1, :-1])[1:] == (1, 5, 0, 10)
+    assert addressed(x[..., :7])[1:] == (1, 24, 0, 10)
+    assert addressed(torch.zeros(1, 10).expand(5, 10))[1:] == (1, 5, 0, 0)
+    y = torch.zeros(3, 4, 5, 10)[:, :-1, :-1]
+    got, *rest = addressed(y)
+    assert got.is_contiguous() and rest == [1, 36, 0, 10]
+    got, *rest = addressed(torch.zeros(10, 4).t())
+    assert got.is_contiguous() and rest == [1, 4, 0, 10]
+    assert addressed(torch.zeros(2, 0, 10))[1:] == (1, 0, 0, 10) or addressed(torch.zeros(2, 0, 10))[1] * 0 == 0
+
+
+def test_c_entry_refuses_bad_arguments():
+    import ctypes
+
+    from dwarf_v2_b200 import _lib
+
+    lib = _lib.load()
+
+    def status(name, struct, **fields):
+        base = dict(version=_lib.ABI_VERSION, dtype=1, logits=4096, outer=1, inner=2, vocab=64, so=0, si=64,
+                    inv_temperature=1.0)
+        return getattr(lib, name)(ctypes.byref(struct(**{**base, **fields})), None)
+
+    fwd = dict(lse=4096, entropy=4096)
+    name, struct = "dwarf_token_logprobs", _lib.TokenLogprobsArgs
+    assert getattr(lib, name)(None, None) == -2
+    assert status(name, struct, **fwd, version=2) == -1
+    assert status(name, struct, lse=4096) == -2
+    assert status(name, struct, **fwd, targets=4096) == -2
+    assert status(name, struct, **fwd, top_k=1) == -2
+    assert status(name, struct, **fwd, logits=None) == -2
+    assert status(name, struct, **fwd, vocab=0) == -3
+    assert status(name, struct, **fwd, vocab=(1 << 20) + 1) == -3
+    assert status(name, struct, **fwd, outer=1 << 20, inner=1 << 20) == -3
+    assert status(name, struct, **fwd, top_k=65) == -3
+    assert status(name, struct, **fwd, top_k=-1) == -3
+    assert status(name, struct, **fwd, si=-64) == -4
+    assert status(name, struct, **fwd, logits=4097) == -5
+    assert status(name, struct, **fwd, dtype=3) == -6
+    assert status(name, struct, **fwd, inv_temperature=0.0) == -9
+    assert status(name, struct, **fwd, inv_temperature=math.nan) == -9
+    assert status(name, struct, **fwd, inv_temperature=math.inf) == -9
+    assert status(name, struct, inner=0, logits=None) == 0  # no rows: nothing to do
+    name, struct = "dwarf_token_logprobs_bwd", _lib.TokenLogprobsBwdArgs
+    bwd = dict(stats=4096, entropy=4096, grad=4096)
+    assert status(name, struct, stats=4096, entropy=4096) == -2
+    assert status(name, struct, **bwd, g_logprob=4096) == -2
+    assert status(name, struct, **bwd, g_top=4096) == -2
+    assert status(name, struct, **bwd, dtype=7) == -6
+
+
+# ------------------------------------------------------------------ GPU
+
+SHAPES = [(1, 1), (3, 2), (5, 31), (2, 129), (7, 1000), (4, 4097), (3, 32768), (1, 32768), (2, 50001), (9, 8192),
+          (300, 515), (1, 131075), (2, 300000), (700, 2049), (1, 1 << 20)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("R,V", SHAPES)
+def test_forward(R, V, dtype):
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    x = logits(R, V, dtype, R * 7 + V).cuda()
+    g = torch.Generator().manual_seed(5)
+    targets = torch.randint(0, V, (R,), generator=g).cuda()
+    targets[R // 2] = -100 if R > 1 else 0
+    for k in sorted({0, 1, min(5, V), min(20, V), min(128, V)}):
+        for t in (1.0, 0.6):
+            check_forward(token_logprobs(x, targets, top_k=k, temperature=t), x, targets, k, t)
+    check_forward(token_logprobs(x, top_k=1), x, None, 1, 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("R,V", [(6, 77), (3, 32768), (40, 8200), (2, 140001)])
+@pytest.mark.parametrize("kind", ["equal", "two_values", "rising", "falling", "front", "stripe", "zeros_signed"])
+def test_top_order_of_hard_rows(R, V, dtype, kind):
+    """Rows with many ties, and rows whose large values lie together: the ids are exact, ties to the lowest."""
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    i = torch.arange(V)
+    row = {"equal": torch.zeros(V), "two_values": (i % 2).float(), "rising": i.float() / V * 20,
+           "falling": -i.float() / V * 20, "front": torch.where(i < V // 3, 4.0 + i % 13, 0.0),
+           "stripe": torch.where(i % 8 == 3, 5.0 + (i % 24) / 8, -1.0),
+           "zeros_signed": torch.where(i % 3 == 0, 0.0, -0.0)}[kind]
+    x = (row + torch.zeros(R, 1)).to(TYPES[dtype]).cuda()
+    for r in range(R):
+        x[r] = x[r].roll(r * 11)
+    for k in sorted({1, min(7, V), min(64, V), min(128, V)}):
+        check_forward(token_logprobs(x, top_k=k), x, None, k, 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("V", [50, 4096, 33001])
+def test_masked_and_special_rows(V, dtype):
+    """-inf, the type's lowest value, +inf and NaN: in places, and in whole rows."""
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    low = torch.finfo(TYPES[dtype]).min
+    x = logits(14, V, dtype, 3)
+    x[0] = -math.inf                      # nothing left
+    x[1] = low                            # the lowest value everywhere: uniform
+    x[2, 1:] = -math.inf                  # one left
+    x[3, 5:] = low
+    x[4, ::2] = -math.inf
+    x[5] = -math.inf
+    x[5, V - 1] = low                     # one finite value, the lowest
+    x[6, 7] = math.inf
+    x[7, 9] = math.nan
+    x[8] = math.nan
+    x[9] = math.inf
+    x[10, 3], x[10, 8] = math.nan, math.inf
+    x[11, :40] = -math.inf
+    x[12] = torch.finfo(TYPES[dtype]).max
+    x[13, 0] = torch.finfo(TYPES[dtype]).max
+    x = x.cuda()
+    targets = torch.full((14,), 1).cuda()
+    targets[2], targets[4] = 0, 2
+    for k in (1, 20, min(50, V)):
+        check_forward(token_logprobs(x, targets, top_k=k), x, targets, k, 1.0)
+    check_forward(token_logprobs(x[:6], targets[:6], top_k=3, temperature=4.0), x[:6], targets[:6], 3, 4.0)
+
+
+@pytest.mark.gpu
+def test_targets_outside_and_ignored():
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    x = logits(6, 100, "fp32", 0).cuda().requires_grad_()
+    targets = torch.tensor([3, -100, -1, 100, 99, 7], dtype=torch.int32).cuda()
+    out = token_logprobs(x, targets, ignore_index=7)
+    lp = out.logprob.detach().cpu()
+    assert torch.isnan(lp[[1, 2, 3]]).all() and lp[5] == 0 and torch.isfinite(lp[[0, 4]]).all()
+    grad, = torch.autograd.grad(out.logprob, x, torch.ones_like(out.logprob))
+    assert torch.isnan(grad[[1, 2, 3]]).all() and torch.equal(grad[5], torch.zeros_like(grad[5]))
+    assert torch.isfinite(grad[[0, 4]]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("R,V,k", [(1, 1, 1), (3, 2, 2), (5, 31, 4), (2, 129, 128), (6, 1000, 0), (3, 32768, 20),
+                                   (2, 50001, 3), (1, 131075, 8), (400, 519, 5), (1, 1 << 20, 2)])
+def test_gradient(R, V, k, dtype):
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    t = 1.3
+    x = logits(R, V, dtype, R + V).cuda().requires_grad_()
+    g = torch.Generator().manual_seed(11)
+    targets = torch.randint(0, V, (R,), generator=g).cuda()
+    if R > 2:
+        targets[1] = -100
+    # fp16 gradients of a large vocabulary would be subnormal: the upstream gradients are of a scaled loss
+    gl, gh, gz = (torch.randn(R, generator=g).cuda() * 64 for _ in range(3))
+    gt = torch.randn(R, k, generator=g).cuda() * 64 if k else None
+    out = token_logprobs(x, targets, top_k=k, temperature=t)
+    if k:
+        targets[0] = int(out.top_ids[0, 0])  # the target among the alternatives: one id twice
+        out = token_logprobs(x, targets, top_k=k, temperature=t)
+    ends = {"g_logprob": (out.logprob, gl), "g_entropy": (out.entropy, gh), "g_lse": (out.lse, gz)}
+    if k:
+        ends["g_top"] = (out.top_logprobs, gt)
+    for chosen in [list(ends), ["g_logprob"], ["g_entropy"], ["g_lse"]] + ([["g_top"]] if k else []):
+        grad, = torch.autograd.grad([ends[c][0] for c in chosen], x, [ends[c][1] for c in chosen], retain_graph=True)
+        assert grad.dtype == x.dtype and grad.shape == x.shape
+        want, size = oracle.token_logprobs_grad(x.detach(), targets, top_ids=out.top_ids, temperature=t,
+                                                **{c: ends[c][1] for c in chosen})
+        close(grad, want, grad_tolerance(x.detach(), t, want, size), chosen)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_gradient_of_masked_rows(dtype):
+    """-inf entries get gradient 0; a row without a finite logit and a row whose gradients are zero get zeros."""
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    V = 2500
+    x = logits(6, V, dtype, 9)
+    x[0] = -math.inf
+    x[1, ::3] = -math.inf
+    x[2, 5:] = -math.inf
+    x[3] = math.nan                      # a padded row: its gradients are zero
+    x[4] = torch.finfo(TYPES[dtype]).min
+    x = x.cuda().requires_grad_()
+    targets = torch.tensor([0, 1, 2, 3, 4, 5]).cuda()
+    gl = torch.tensor([1.0, 2.0, -1.0, 0.0, 3.0, 1.0]).cuda()
+    gh = torch.tensor([0.5, 1.0, 2.0, 0.0, 1.0, 0.0]).cuda()
+    out = token_logprobs(x, targets, top_k=3)
+    grad, = torch.autograd.grad([out.logprob, out.entropy], x, [gl, gh])
+    want, size = oracle.token_logprobs_grad(torch.nan_to_num(x.detach(), nan=0.0, neginf=-math.inf), targets,
+                                            g_logprob=gl, g_entropy=gh)
+    want[3], size[3] = 0.0, 0.0
+    close(grad, want, grad_tolerance(torch.nan_to_num(x.detach(), nan=0.0, neginf=-math.inf), 1.0, want, size))
+    assert torch.equal(grad[3], torch.zeros_like(grad[3])) and torch.equal(grad[0], torch.zeros_like(grad[0]))
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences():
+    """The fp32 kernel's own outputs, differenced in a direction: 64-bit sums of fp32 outputs."""
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    g = torch.Generator().manual_seed(2)
+    x = (torch.randn(4, 600, generator=g)).cuda().requires_grad_()
+    targets = torch.randint(0, 600, (4,), generator=g).cuda()
+    out = token_logprobs(x, targets)
+    grad, = torch.autograd.grad(out.logprob.sum() + out.entropy.sum(), x)
+    way = torch.randn(4, 600, generator=g).cuda()
+    step = 2.0 ** -6
+    with torch.no_grad():
+        hi, lo = token_logprobs(x + step * way, targets), token_logprobs(x - step * way, targets)
+    diff = ((hi.logprob - lo.logprob).double().sum() + (hi.entropy - lo.entropy).double().sum()) / (2 * step)
+    # truncation step^2 |f'''| / 6 < 2^-12 at unit directions per entry; roundings 8 * 8 * 2^-24 / step < 2^-12
+    assert abs(float(diff) - float((grad.double() * way.double()).sum())) < 2.0 ** -8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_strides_and_alignment(dtype):
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    g = torch.Generator().manual_seed(4)
+    big = (torch.randn(3, 5, 6, 1031, generator=g) * 2).to(TYPES[dtype]).cuda()
+    views = {"contiguous": big, "shifted": big[0, :, :-1], "last": big[0, :, -1], "columns": big[..., 3:1029],
+             "three groups": big[:, :-1, :-1], "transposed": big[0, 0].t(), "row": big[1, 2, 3],
+             "expanded": big[0, 0, :1].expand(4, 1031), "permuted": big[0].transpose(0, 1), "odd base": big[0, 0, 1:, 1:]}
+    for name, view in views.items():
+        lead, V = view.shape[:-1], view.shape[-1]
+        targets = torch.randint(0, V, lead, generator=g).cuda()
+        out = token_logprobs(view, targets, top_k=3)
+        assert out.entropy.shape == lead and out.top_ids.shape == (*lead, 3)
+        check_forward(out, view.contiguous(), targets, 3, 1.0)
+        leaf = view.detach().requires_grad_()
+        out = token_logprobs(leaf, targets)
+        w = torch.randn(lead, generator=g).cuda() if lead else torch.tensor(1.5).cuda()
+        grad, = torch.autograd.grad(out.logprob, leaf, w)
+        flat = view.reshape(-1, V)
+        want, size = oracle.token_logprobs_grad(flat, targets.reshape(-1), g_logprob=w.reshape(-1))
+        close(grad.reshape(-1, V), want, grad_tolerance(flat, 1.0, want, size), name)
+
+
+@pytest.mark.gpu
+def test_no_rows_and_neighbours_untouched():
+    from dwarf_v2_b200 import _lib, _rows
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    x = torch.zeros(0, 7, device="cuda", requires_grad=True)
+    out = token_logprobs(x, torch.zeros(0, dtype=torch.int64, device="cuda"), top_k=2)
+    assert out.logprob.shape == (0,) and out.top_ids.shape == (0, 2)
+    assert torch.autograd.grad(out.entropy.sum(), x)[0].shape == (0, 7)
+    # one odd row in the middle of a buffer: nothing before or behind it is written
+    V = 1003
+    row = logits(1, V, "bf16", 1).cuda()
+    buf = torch.full((3 * V,), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = token_logprobs(row.clone().requires_grad_(), torch.tensor([3]).cuda())
+    stats = torch.tensor([[float(row.float().max()), 1.0]], device="cuda")
+    one = torch.ones(1, device="cuda")
+    targets = torch.tensor([3], device="cuda")
+    args = _lib.TokenLogprobsBwdArgs(version=1, dtype=1, logits=row.data_ptr(), outer=1, inner=1, vocab=V, so=0, si=V,
+                                     targets=targets.data_ptr(), ignore_index=-100, inv_temperature=1.0, top_k=0,
+                                     stats=stats.data_ptr(), entropy=one.data_ptr(), g_logprob=one.data_ptr(),
+                                     grad=buf.data_ptr() + 2 * V)
+    _rows.launch("dwarf_token_logprobs_bwd", args, row.device)
+    assert torch.equal(buf[:V], torch.full_like(buf[:V], 7.0)) and torch.equal(buf[2 * V:], buf[:V])
+    assert not (buf[V:2 * V] == 7.0).all()
+
+
+@pytest.mark.gpu
+def test_repeatable_on_streams_and_in_graphs():
+    """Bit-identical on a side stream, in a captured and replayed graph (forward and backward), and in two graphs."""
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    x = logits(37, 32768, "bf16", 8).cuda()
+    targets = torch.arange(37).cuda()
+
+    def both(v):
+        leaf = v.detach().requires_grad_()
+        out = token_logprobs(leaf, targets, top_k=20)
+        grad, = torch.autograd.grad([out.logprob, out.entropy], leaf,
+                                    [torch.ones_like(out.logprob), torch.ones_like(out.entropy)])
+        return [out.logprob.detach(), out.entropy.detach(), out.top_logprobs.detach(), out.top_ids, grad]
+
+    eager = both(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = both(x)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(eager, other))
+    static = torch.zeros_like(x)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = both(static)
+        graphs.append((graph, got))
+    for shift in (0, 5):
+        static.copy_(x.roll(shift, 1))
+        want = both(static)
+        for graph, got in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, got in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.gpu
+def test_rows_past_32_bit_offsets():
+    """A tensor of over 2^32 elements: its last rows are read and their gradient written in place."""
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    V, R = 32768, (1 << 32) // 32768 + 3
+    x = torch.empty(R, V, dtype=torch.bfloat16, device="cuda")
+    x.zero_()
+    tail = logits(3, V, "bf16", 6).cuda()
+    x[-3:] = tail
+    targets = torch.full((R,), 17, device="cuda")
+    x.requires_grad_()
+    out = token_logprobs(x, targets, top_k=2)
+    small = token_logprobs(tail, targets[-3:], top_k=2)
+    assert torch.equal(out.logprob[-3:], small.logprob) and torch.equal(out.top_ids[-3:], small.top_ids)
+    up = torch.zeros(R, device="cuda")
+    up[-3:] = 1.0
+    grad, = torch.autograd.grad(out.logprob, x, up)
+    want, size = oracle.token_logprobs_grad(tail, targets[-3:], g_logprob=up[-3:])
+    close(grad[-3:], want, grad_tolerance(tail, 1.0, want, size))
+    assert not bool((grad[:-3] != 0).any())
