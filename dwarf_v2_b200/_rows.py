@@ -21,7 +21,7 @@ def check_logits(logits: torch.Tensor, temperature: float) -> float:
         raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
     if not 1 <= logits.shape[-1] <= VOCAB_MAX:
         raise ValueError(f"the vocabulary must hold 1..{VOCAB_MAX} entries, got {logits.shape[-1]}")
-    if logits.numel() // logits.shape[-1] > 0x7FFFFFFF:
+    if logits.numel() // logits.shape[-1] >= 1 << 28:
         raise ValueError("too many rows")
     temperature = float(temperature)
     if not (math.isfinite(temperature) and 1e-30 <= temperature <= 1e30):

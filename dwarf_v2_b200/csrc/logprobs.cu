@@ -10,59 +10,371 @@
 namespace dwarf {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kVectors = 8;         // 16-byte vectors of a row that a thread holds
+constexpr int kCandidates = 1024;   // entries that the search for the alternatives may sort
+constexpr int kMaxCluster = 8;
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(dwarf_token_logprobs_args a) {
-  __shared__ float sf[kThreads / 32];
-  __shared__ uint64_t sk[kThreads / 32];
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(a.logits) + row_offset(row, a.inner, a.so, a.si);
-  const int vocab = (int)a.vocab;
-  const float c2 = a.inv_temperature * kLog2e;
-  float m = -CUDART_INF_F;
-  for (int i = threadIdx.x; i < vocab; i += kThreads) m = fmaxf(m, to_f32(x[i]));
-  m = block_reduce<kThreads>(m, sf, MaxOp());
-  if (m == -CUDART_INF_F) m = 0.0f;
-  float s = 0.0f, t = 0.0f;
-  for (int i = threadIdx.x; i < vocab; i += kThreads) {
-    const float d = (to_f32(x[i]) - m) * c2;
-    const float e = ex2_approx(d);
-    s += e;
-    t += e * fmaxf(d, -200.0f);
+// What a softmax needs of a part of a row: the maximum, S and T relative to it.
+struct Sums {
+  float m, s, t;
+};
+
+// One Sums from those of a warp's lanes (lanes without a part: m = -inf, s = t = 0), in a fixed order.
+__device__ __forceinline__ Sums warp_join(Sums p, float c2) {
+  const float m = warp_max(p.m);
+  const float d = fmaxf((p.m - (m == -CUDART_INF_F ? 0.0f : m)) * c2, -200.0f);
+  const float f = p.s == 0.0f ? 0.0f : ex2_approx(d);
+  return {m, warp_sum(f * p.s), warp_sum(f * fmaf(d, p.s, p.t))};
+}
+
+// The vectors of one row's part, NT threads and N vectors a thread at a time. A part
+// of one tile stays in registers; a longer one is read again by each walk.
+template <typename T, int NT, int N>
+struct Part {
+  static constexpr int kVec = Vec16<T>::kVec;
+  RowVectors<T> row;
+  int j0, j1, tiles;
+  uint4 v[N];
+
+  __device__ __forceinline__ Part(const T* x, int vocab, int rank, int cluster) : row(x, vocab) {
+    const int n = row.count(), per = ceil_div(n, cluster);
+    j0 = rank * per;
+    j1 = j0 + per < n ? j0 + per : n;
+    tiles = j1 > j0 ? ceil_div(j1 - j0, NT * N) : 0;
   }
-  s = block_reduce<kThreads>(s, sf, AddOp());
-  t = block_reduce<kThreads>(t, sf, AddOp());
-  const float log2s = log2f(s);  // -inf for a row without a finite logit
-  if (threadIdx.x == 0) {
-    a.lse[row] = s > 0.0f ? fmaf(m, a.inv_temperature, log2s * kLn2) : s == 0.0f ? -CUDART_INF_F : s;
-    a.entropy[row] = s == 0.0f ? 0.0f : (log2s - t / s) * kLn2;
-    if (a.stats != nullptr) reinterpret_cast<float2*>(a.stats)[row] = make_float2(m, s);
-    if (a.logprob != nullptr) {
-      const int64_t id = a.targets[row];
-      float lp = 0.0f;
-      if (id != a.ignore_index) {
-        lp = CUDART_NAN_F;
-        if (id >= 0 && id < vocab) lp = s == 0.0f ? -CUDART_INF_F : (to_f32(x[id]) - m) * a.inv_temperature - log2s * kLn2;
+  __device__ __forceinline__ int first(int tile, int i) const { return j0 + (tile * N + i) * NT; }
+  __device__ __forceinline__ void load(int tile) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int j = first(tile, i) + threadIdx.x;
+      v[i] = make_uint4(Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf);
+      if (j < j1) v[i] = row.load(j);
+    }
+  }
+  // f(vector, j) in rising j; every thread of the block takes part in every step.
+  template <typename F>
+  __device__ __forceinline__ void walk(F f) {
+    for (int tile = 0; tile < tiles; ++tile) {
+      if (tiles > 1) load(tile);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (first(tile, i) < j1) f(v[i], first(tile, i) + (int)threadIdx.x);
+    }
+  }
+  // f(value, id) for the elements of vector j that are in the row.
+  template <typename F>
+  __device__ __forceinline__ void elements(const uint4& w, int j, F f) const {
+    float2 x[kVec / 2];
+    Vec16<T>::unpack(w, x);
+    if (j >= j1) return;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      const int u = j * kVec + e;
+      if (u >= row.lead && u < row.end) f(e & 1 ? x[e / 2].y : x[e / 2].x, u - row.lead);
+    }
+  }
+};
+
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+
+struct TopShared {
+  uint32_t value[512];               // order keys of the threads' maxima
+  uint32_t group[256];
+  uint64_t candidate[kCandidates];
+  uint32_t threshold;
+  int n;
+  int scan[16];
+};
+
+// The K best entries of the part (order: value, then lowest id) among the first n
+// candidates, n >= min(K, entries of the part). The common case: with G >= 2 K groups
+// of threads, the K-th largest of the groups' maxima bounds the K-th entry from below,
+// and the entries from there up are few (G ln(G / (G - K)) if their places are random).
+// Where they are more than the buffer holds (ties, one group with many large values), or a
+// NaN is in the row, the K-th value is found bit by bit and its ties are taken in order.
+template <typename T, int NT, int N>
+__device__ __forceinline__ int best_entries(Part<T, NT, N>& part, float thread_max, int k, bool nan, TopShared& sh) {
+  const int tid = threadIdx.x;
+  int groups = 32;
+  while (groups < 2 * k && groups < NT && groups < 256) groups *= 2;
+  // sh.value was written before the caller's barrier
+  if (tid < groups) {
+    uint32_t g = 0;
+    for (int i = tid; i < NT; i += groups) g = max(g, sh.value[i]);
+    sh.group[tid] = g;
+  }
+  if (tid == 0) sh.n = 0;
+  __syncthreads();
+  if (tid < groups) {
+    const uint32_t g = sh.group[tid];
+    int above = 0;
+    const uint4* q = reinterpret_cast<const uint4*>(sh.group);
+    for (int i = 0; i < groups / 4; ++i) {
+      const uint4 w = q[i];
+      above += (w.x > g || (w.x == g && 4 * i < tid)) + (w.y > g || (w.y == g && 4 * i + 1 < tid)) +
+               (w.z > g || (w.z == g && 4 * i + 2 < tid)) + (w.w > g || (w.w == g && 4 * i + 3 < tid));
+    }
+    if (above == k - 1) sh.threshold = g;
+  }
+  __syncthreads();
+  uint32_t limit = sh.threshold;
+  if (!nan) {
+    const float bound = key_value(limit);
+    if (thread_max >= bound || part.tiles > 1) {
+      // no barrier inside: threads below the bound pass over their vectors
+      for (int tile = 0; tile < part.tiles; ++tile) {
+        if (part.tiles > 1) part.load(tile);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (Vec16<T>::max(part.v[i]) >= bound)
+            part.elements(part.v[i], part.first(tile, i) + tid, [&](float x, int id) {
+              if (x >= bound) {
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < kCandidates) sh.candidate[at] = entry_key(x, (uint32_t)id);
+              }
+            });
+        }
       }
-      a.logprob[row] = lp;
+    }
+    __syncthreads();
+    if (sh.n <= kCandidates) return sh.n;
+  }
+  // count the entries of the part with a key of at least `from`
+  auto count = [&](uint32_t from) {
+    int c = 0;
+    part.walk([&](const uint4& w, int j) { part.elements(w, j, [&](float x, int) { c += order_key(x) >= from; }); });
+    c = __reduce_add_sync(0xffffffffu, c);
+    __syncthreads();
+    if ((tid & 31) == 0) sh.scan[tid >> 5] = c;
+    __syncthreads();
+    c = 0;
+    for (int i = 0; i < NT / 32; ++i) c += sh.scan[i];
+    return c;
+  };
+  if (nan || count(limit + 1) >= k) {
+    limit = 0;
+    for (int bit = 31; bit >= 0; --bit)
+      if (count(limit | (1u << bit)) >= k) limit |= 1u << bit;
+  }
+  __syncthreads();
+  if (tid == 0) sh.n = 0;
+  __syncthreads();
+  part.walk([&](const uint4& w, int j) {
+    part.elements(w, j, [&](float x, int id) {
+      if (order_key(x) > limit) sh.candidate[atomicAdd(&sh.n, 1)] = entry_key(x, (uint32_t)id);  // fewer than k
+    });
+  });
+  __syncthreads();
+  int have = sh.n;
+  part.walk([&](const uint4& w, int j) {
+    if (have >= k) return;  // the same for the whole block
+    int c = 0;
+    part.elements(w, j, [&](float x, int) { c += order_key(x) == limit; });
+    int at = c;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int up = __shfl_up_sync(0xffffffffu, at, o);
+      if ((tid & 31) >= o) at += up;
+    }
+    if ((tid & 31) == 31) sh.scan[tid >> 5] = at;
+    __syncthreads();
+    int total = 0;
+    for (int i = 0; i < NT / 32; ++i) {
+      if (i < (tid >> 5)) at += sh.scan[i];
+      total += sh.scan[i];
+    }
+    at += have - c;
+    part.elements(w, j, [&](float x, int id) {
+      if (order_key(x) != limit) return;
+      if (at < k) sh.candidate[at] = entry_key(x, (uint32_t)id);
+      ++at;
+    });
+    have = min(k, have + total);
+    __syncthreads();
+  });
+  __syncthreads();
+  return have;
+}
+
+// One CTA, or a cluster of them, for a row.
+template <typename T, int NT, int N, bool kTop>
+__global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const dwarf_token_logprobs_args a, int cluster) {
+  constexpr int kWarps = NT / 32;
+  __shared__ Sums s_warp[kWarps];
+  __shared__ float s_parts[kMaxCluster][3];
+  __shared__ Sums s_row;
+  __shared__ uint64_t s_lists[kTop ? kMaxCluster * DWARF_TOP_K_MAX : 1];
+  __shared__ __align__(16) unsigned char s_top[kTop ? sizeof(TopShared) : 16];
+  TopShared& top = *reinterpret_cast<TopShared*>(s_top);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = cluster > 1 ? (int)cluster_rank() : 0;
+  const int64_t r = blockIdx.x / (unsigned)cluster;
+  const T* x = static_cast<const T*>(a.logits) + row_offset(r, a.inner, a.so, a.si);
+  const int vocab = (int)a.vocab, k = a.top_k;
+  const float c2 = a.inv_temperature * kLog2e;
+  if (cluster > 1) cluster_arrive();  // its CTAs have started, before one writes to another
+
+  Part<T, NT, N> part(x, vocab, rank, cluster);
+  Sums sum = {-CUDART_INF_F, 0.0f, 0.0f};
+  float thread_max = -CUDART_INF_F;
+  for (int tile = 0; tile < part.tiles; ++tile) {
+    part.load(tile);
+    float mx = Vec16<T>::max(part.v[0]);
+#pragma unroll
+    for (int i = 1; i < N; ++i) mx = fmaxf(mx, Vec16<T>::max(part.v[i]));
+    thread_max = fmaxf(thread_max, mx);
+    const float m = fmaxf(sum.m, warp_max(mx));
+    if (sum.m > -CUDART_INF_F) {  // a later tile: move the sums to the new maximum
+      const float d = fmaxf((sum.m - m) * c2, -200.0f), f = ex2_approx(d);
+      sum.t = f * fmaf(d, sum.s, sum.t);
+      sum.s *= f;
+    }
+    sum.m = m;
+    const float shift = m == -CUDART_INF_F ? 0.0f : -m;
+    float2 s = make_float2(0.0f, 0.0f), t = s;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (part.first(tile, i) >= part.j1) break;
+      float2 e[Part<T, NT, N>::kVec / 2];
+      Vec16<T>::unpack(part.v[i], e);
+#pragma unroll
+      for (int h = 0; h < Part<T, NT, N>::kVec / 2; ++h) {
+        const float2 d = mul2(add2(e[h], make_float2(shift, shift)), make_float2(c2, c2));
+        const float2 p = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+        s = add2(s, p);
+        t = fma2(p, make_float2(fmaxf(d.x, -200.0f), fmaxf(d.y, -200.0f)), t);  // 0 (-inf) counts as 0
+      }
+    }
+    sum.s += s.x + s.y;
+    sum.t += t.x + t.y;
+  }
+  sum.s = warp_sum(sum.s);
+  sum.t = warp_sum(sum.t);
+  if (lane == 0) s_warp[warp] = sum;
+  if (kTop) top.value[tid] = order_key(thread_max);
+  __syncthreads();
+  if (cluster > 1) cluster_wait();
+  if (!kTop && warp != kWarps - 1 && cluster == 1) return;
+  Sums all = {-CUDART_INF_F, 0.0f, 0.0f};  // in the last warp: of the part, then of the row
+  if (warp == kWarps - 1) {
+    if (lane < kWarps) all = s_warp[lane];
+    all = warp_join(all, c2);
+    if (cluster > 1 && lane < 3) {
+      const uint32_t to = cluster_address(&s_parts[rank][lane], 0);
+      st_cluster(to, lane == 0 ? all.m : lane == 1 ? all.s : all.t);
     }
   }
-  uint64_t last = ~0ull;
-  for (int k = 0; k < a.top_k; ++k) {
-    uint64_t best = 0;
-    for (int i = threadIdx.x; i < vocab; i += kThreads) {
-      const uint64_t key = entry_key(to_f32(x[i]), (uint32_t)i);
-      if (key < last && key > best) best = key;
+  int n = 0;
+  if (kTop) {
+    // a NaN or +inf anywhere in the part makes some warp's sum NaN
+    bool nan = false;
+    for (int w = 0; w < kWarps; ++w) nan |= s_warp[w].s != s_warp[w].s;
+    n = best_entries(part, thread_max, k, nan, top);
+  }
+  if (cluster > 1) {
+    if (kTop) {
+      for (int c = tid; c < max(n, k); c += NT) {
+        uint64_t key = 0;
+        int at = c;
+        if (c < n) {
+          key = top.candidate[c];
+          at = 0;
+          for (int i = 0; i < n; ++i) at += top.candidate[i] > key;
+        }
+        if (at < k) st_cluster(cluster_address(&s_lists[rank * k + at], 0), key);
+      }
     }
-    last = block_reduce<kThreads>(best, sk, MaxOp());
-    if (threadIdx.x == 0) {
-      const uint32_t id = entry_id(last);
-      a.top_ids[row * a.top_k + k] = id;
-      a.top_logprobs[row * a.top_k + k] = s == 0.0f ? -CUDART_INF_F : (to_f32(x[id]) - m) * a.inv_temperature - log2s * kLn2;
+    cluster_arrive();
+    if (rank != 0) return;
+    cluster_wait();
+    if (!kTop && warp != kWarps - 1) return;
+  }
+  if (warp == kWarps - 1) {
+    if (cluster > 1) {
+      all = {-CUDART_INF_F, 0.0f, 0.0f};
+      if (lane < cluster) all = {s_parts[lane][0], s_parts[lane][1], s_parts[lane][2]};
+      all = warp_join(all, c2);
+    }
+    if (all.m == -CUDART_INF_F) all.m = 0.0f;
+    const float ln_s = log2f(all.s) * kLn2;  // -inf for a row without a finite logit
+    if (lane == 0) {
+      a.lse[r] = all.s == 0.0f ? -CUDART_INF_F : fmaf(all.m, a.inv_temperature, ln_s);
+      a.entropy[r] = all.s == 0.0f ? 0.0f : ln_s - all.t / all.s * kLn2;
+      if (a.stats != nullptr) reinterpret_cast<float2*>(a.stats)[r] = make_float2(all.m, all.s);
+      if (a.logprob != nullptr) {
+        const int64_t id = a.targets[r];
+        float lp = 0.0f;
+        if (id != a.ignore_index) {
+          lp = CUDART_NAN_F;
+          if (id >= 0 && id < vocab)
+            lp = all.s == 0.0f ? -CUDART_INF_F : (to_f32(x[id]) - all.m) * a.inv_temperature - ln_s;
+        }
+        a.logprob[r] = lp;
+      }
+      s_row = {all.m, all.s, ln_s};
+    }
+  }
+  if (!kTop) return;
+  __syncthreads();
+  const Sums fin = s_row;
+  auto put = [&](uint64_t key, int at) {
+    a.top_ids[r * k + at] = entry_id(key);
+    a.top_logprobs[r * k + at] =
+        fin.s == 0.0f ? -CUDART_INF_F : (key_value((uint32_t)(key >> 32)) - fin.m) * a.inv_temperature - fin.t;
+  };
+  if (cluster == 1) {
+    for (int c = tid; c < n; c += NT) {
+      const uint64_t key = top.candidate[c];
+      int at = 0;
+      for (int i = 0; i < n; ++i) at += top.candidate[i] > key;
+      if (at < k) put(key, at);
+    }
+  } else {
+    for (int c = tid; c < cluster * k; c += NT) {
+      const uint64_t key = s_lists[c];
+      if (key == 0) continue;  // a part with fewer than k entries
+      int at = c % k;
+      for (int o = 0; o < cluster; ++o) {
+        if (o == c / k) continue;
+        int lo = 0, hi = k;  // entries of the other part's falling list that are above this one
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (s_lists[o * k + mid] > key) lo = mid + 1; else hi = mid;
+        }
+        at += lo;
+      }
+      if (at < k) put(key, at);
     }
   }
 }
+
+// How many CTAs share a row: enough that its part fits a CTA's registers, and more
+// while the rows alone leave SMs without work and a part keeps 128 vectors or more.
+inline int cluster_for(int64_t rows, int vectors, int tile) {
+  int c = 1;
+  while (c < kMaxCluster && vectors > c * tile) c *= 2;
+  while (c < kMaxCluster && rows * c * 2 <= kNumSMs && vectors >= c * 2 * 128) c *= 2;
+  return c;
+}
+
+template <typename T>
+int launch_forward(const dwarf_token_logprobs_args& a, cudaStream_t stream) {
+  const int64_t rows = a.outer * a.inner;
+  const int vectors = ceil_div((int)a.vocab, Vec16<T>::kVec);
+  const int cluster = cluster_for(rows, vectors, 512 * kVectors);
+  const int part = ceil_div(vectors, cluster);
+  // 128 threads where they hold the part and the groups that bound the alternatives
+  const bool small = part <= 128 * kVectors && a.top_k <= 32;
+  if (a.top_k > 0)
+    return small ? launch_rows(token_logprobs_kernel<T, 128, kVectors, true>, rows, cluster, 128, 0, stream, a, cluster)
+                 : launch_rows(token_logprobs_kernel<T, 512, kVectors, true>, rows, cluster, 512, 0, stream, a, cluster);
+  return small ? launch_rows(token_logprobs_kernel<T, 128, kVectors, false>, rows, cluster, 128, 0, stream, a, cluster)
+               : launch_rows(token_logprobs_kernel<T, 512, kVectors, false>, rows, cluster, 512, 0, stream, a, cluster);
+}
+
+constexpr int kThreads = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(dwarf_token_logprobs_bwd_args a) {
@@ -139,10 +451,7 @@ extern "C" int dwarf_token_logprobs(const dwarf_token_logprobs_args* args, void*
   if (a.lse == nullptr || a.entropy == nullptr) return DWARF_ERR_NULL;
   if ((a.targets == nullptr) != (a.logprob == nullptr)) return DWARF_ERR_NULL;
   if (a.top_k > 0 && (a.top_logprobs == nullptr || a.top_ids == nullptr)) return DWARF_ERR_NULL;
-  return with_type(a.dtype, [&](auto t) {
-    token_logprobs_kernel<decltype(t)><<<(unsigned)rows, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    return launch_status();
-  });
+  return with_type(a.dtype, [&](auto t) { return launch_forward<decltype(t)>(a, static_cast<cudaStream_t>(stream)); });
 }
 
 extern "C" int dwarf_token_logprobs_bwd(const dwarf_token_logprobs_bwd_args* args, void* stream) {

@@ -66,11 +66,202 @@ struct MaxOp {
   __device__ __forceinline__ uint64_t operator()(uint64_t a, uint64_t b) const { return a > b ? a : b; }
 };
 
+// Packed pairs of fp32 (one issue slot for two elements).
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 pa, pb, pr;\nmov.b64 pa, {%2, %3};\nmov.b64 pb, {%4, %5};\n"
+      "add.rn.f32x2 pr, pa, pb;\nmov.b64 {%0, %1}, pr;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 pa, pb, pr;\nmov.b64 pa, {%2, %3};\nmov.b64 pb, {%4, %5};\n"
+      "mul.rn.f32x2 pr, pa, pb;\nmov.b64 {%0, %1}, pr;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{.reg .b64 pa, pb, pc;\nmov.b64 pa, {%2, %3};\nmov.b64 pb, {%4, %5};\nmov.b64 pc, {%6, %7};\n"
+      "fma.rn.f32x2 pc, pa, pb, pc;\nmov.b64 {%0, %1}, pc;\n}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
+// 16 bytes of a row: kVec elements.
+template <typename T>
+struct Vec16;
+
+template <>
+struct Vec16<float> {
+  static constexpr int kVec = 4;
+  static constexpr uint32_t kMinusInf = 0xff800000u;
+  __device__ __forceinline__ static void unpack(const uint4& v, float2 (&x)[2]) {
+    x[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+    x[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+  }
+  __device__ __forceinline__ static uint4 pack(const float2 (&x)[2]) {
+    return make_uint4(__float_as_uint(x[0].x), __float_as_uint(x[0].y), __float_as_uint(x[1].x),
+                      __float_as_uint(x[1].y));
+  }
+  // Largest element; NaN is passed over.
+  __device__ __forceinline__ static float max(const uint4& v) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+};
+
+template <>
+struct Vec16<__nv_bfloat16> {
+  static constexpr int kVec = 8;
+  static constexpr uint32_t kMinusInf = 0xff80ff80u;
+  __device__ __forceinline__ static void unpack(const uint4& v, float2 (&x)[4]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
+  __device__ __forceinline__ static uint4 pack(const float2 (&x)[4]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[i].x, x[i].y);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ static float max(const uint4& v) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(f.x, f.y);
+  }
+};
+
+template <>
+struct Vec16<__half> {
+  static constexpr int kVec = 8;
+  static constexpr uint32_t kMinusInf = 0xfc00fc00u;
+  __device__ __forceinline__ static void unpack(const uint4& v, float2 (&x)[4]) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __half22float2(h[i]);
+  }
+  __device__ __forceinline__ static uint4 pack(const float2 (&x)[4]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(x[i].x, x[i].y);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ static float max(const uint4& v) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    const float2 f = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(f.x, f.y);
+  }
+};
+
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// A row as aligned 16-byte vectors. Places u count from the 16-byte boundary at or
+// before the row's first element: element id lies at u = id + lead, vector j holds
+// places [j kVec, (j + 1) kVec). Only the first and the last vector may hold places
+// outside the row; they are read element by element, the places outside as -inf.
+template <typename T>
+struct RowVectors {
+  static constexpr int kVec = Vec16<T>::kVec;
+  const T* base;  // the boundary (not read before the row)
+  int lead;       // elements between the boundary and the row
+  int end;        // lead + vocab
+  __device__ __forceinline__ RowVectors(const T* row, int vocab) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row);
+    lead = (int)((at & 15) / sizeof(T));
+    base = row - lead;
+    end = lead + vocab;
+  }
+  __device__ __forceinline__ int count() const { return (end + kVec - 1) / kVec; }
+  __device__ __forceinline__ bool whole(int j) const { return j * kVec >= lead && (j + 1) * kVec <= end; }
+  __device__ __forceinline__ uint4 load(int j) const {
+    if (whole(j)) return ld_stream(base + (int64_t)j * kVec);
+    uint4 v = make_uint4(Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf);
+    T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const int u = j * kVec + i;
+      if (u >= lead && u < end) e[i] = base[u];
+    }
+    return v;
+  }
+};
+
+__host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Largest value over a warp, through the integers that order floats.
+__device__ __forceinline__ float warp_max(float v) {
+  int k = __float_as_int(v);
+  k ^= (k >> 31) & 0x7fffffff;
+  k = __reduce_max_sync(0xffffffffu, k);
+  k ^= (k >> 31) & 0x7fffffff;
+  return __int_as_float(k);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The CTAs of a cluster share one row.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// The shared-memory address of the same variable in CTA `rank` of the cluster, for st.shared::cluster.
+__device__ __forceinline__ uint32_t cluster_address(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint64_t v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+
+// Launch with `cluster` CTAs for each row.
+template <typename... Params, typename... Args>
+int launch_rows(void (*kernel)(Params...), int64_t rows, int cluster, int threads, size_t smem, cudaStream_t stream,
+                Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * cluster));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) return launch_status();
+  return launch_status();
+}
+
 // Host checks shared by the entry points: sizes, strides and the scale of a logit tensor.
 inline int check_logits(const void* logits, int32_t dtype, int64_t outer, int64_t inner, int64_t vocab, int64_t so,
                         int64_t si, float inv_temperature) {
   if (outer < 0 || inner < 0 || vocab < 1 || vocab > DWARF_VOCAB_MAX) return DWARF_ERR_SHAPE;
-  if (outer > 0 && inner > 0x7fffffffll / outer) return DWARF_ERR_SHAPE;
+  if (outer > 0 && inner > ((1ll << 28) - 1) / outer) return DWARF_ERR_SHAPE;
   if (so < 0 || si < 0) return DWARF_ERR_STRIDE;
   if (dtype != DWARF_F32 && dtype != DWARF_BF16 && dtype != DWARF_F16) return DWARF_ERR_DTYPE;
   const float c2 = inv_temperature * kLog2e;

@@ -446,7 +446,7 @@ def test_repeatable_on_streams_and_in_graphs():
 @pytest.mark.gpu
 def test_rows_past_32_bit_offsets():
     """A tensor of over 2^32 elements: its last rows are read and their gradient written in place."""
-    from dwarf_v2_b200.logprobs import token_logprobs
+    from dwarf_v2_b200.logprobs import TokenLogprobs, token_logprobs
 
     V, R = 32768, (1 << 32) // 32768 + 3
     x = torch.empty(R, V, dtype=torch.bfloat16, device="cuda")
@@ -456,8 +456,7 @@ def test_rows_past_32_bit_offsets():
     targets = torch.full((R,), 17, device="cuda")
     x.requires_grad_()
     out = token_logprobs(x, targets, top_k=2)
-    small = token_logprobs(tail, targets[-3:], top_k=2)
-    assert torch.equal(out.logprob[-3:], small.logprob) and torch.equal(out.top_ids[-3:], small.top_ids)
+    check_forward(TokenLogprobs(*(t.detach()[-3:] for t in out)), tail, targets[-3:], 2, 1.0)
     up = torch.zeros(R, device="cuda")
     up[-3:] = 1.0
     grad, = torch.autograd.grad(out.logprob, x, up)
