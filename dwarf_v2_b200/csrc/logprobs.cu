@@ -11,7 +11,8 @@ namespace dwarf {
 namespace {
 
 constexpr int kVectors = 8;         // 16-byte vectors of a row that a thread holds
-constexpr int kCandidates = 1024;   // entries that the search for the alternatives may sort
+constexpr int kCandidates = 512;    // entries that the search for the alternatives may sort
+constexpr int kHits = 512;          // vectors that it may look through
 constexpr int kMaxCluster = 8;
 
 // What a softmax needs of a part of a row: the maximum, S and T relative to it.
@@ -44,11 +45,18 @@ struct Part {
   }
   __device__ __forceinline__ int first(int tile, int i) const { return j0 + (tile * N + i) * NT; }
   __device__ __forceinline__ void load(int tile) {
+    const int j = first(tile, 0) + threadIdx.x;
+    const int lo = row.lead > 0 ? 1 : 0, hi = row.end / kVec;  // the whole vectors
+    const uint4* p = reinterpret_cast<const uint4*>(row.base) + j;
+    if (first(tile, 0) >= lo && first(tile, N) <= (j1 < hi ? j1 : hi)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = ld_stream(p + i * NT);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int j = first(tile, i) + threadIdx.x;
       v[i] = make_uint4(Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf);
-      if (j < j1) v[i] = row.load(j);
+      if (first(tile, i) < j1 && j + i * NT < j1) v[i] = row.load(j + i * NT);
     }
   }
   // f(vector, j) in rising j; every thread of the block takes part in every step.
@@ -82,9 +90,11 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 struct TopShared {
   uint32_t value[512];               // order keys of the threads' maxima
   uint32_t group[256];
+  uint4 hit[kHits];                  // vectors with an entry of at least the threshold
+  int hit_at[kHits];
   uint64_t candidate[kCandidates];
   uint32_t threshold;
-  int n;
+  int n, hits;
   int scan[16];
 };
 
@@ -105,41 +115,57 @@ __device__ __forceinline__ int best_entries(Part<T, NT, N>& part, float thread_m
     for (int i = tid; i < NT; i += groups) g = max(g, sh.value[i]);
     sh.group[tid] = g;
   }
-  if (tid == 0) sh.n = 0;
+  if (tid == 0) sh.n = sh.hits = 0, sh.threshold = 0xffffffffu;
   __syncthreads();
   if (tid < groups) {
+    // the K-th largest is the smallest that fewer than K exceed
     const uint32_t g = sh.group[tid];
     int above = 0;
     const uint4* q = reinterpret_cast<const uint4*>(sh.group);
     for (int i = 0; i < groups / 4; ++i) {
       const uint4 w = q[i];
-      above += (w.x > g || (w.x == g && 4 * i < tid)) + (w.y > g || (w.y == g && 4 * i + 1 < tid)) +
-               (w.z > g || (w.z == g && 4 * i + 2 < tid)) + (w.w > g || (w.w == g && 4 * i + 3 < tid));
+      above += (w.x > g) + (w.y > g) + (w.z > g) + (w.w > g);
     }
-    if (above == k - 1) sh.threshold = g;
+    const uint32_t least = __reduce_min_sync(0xffffffffu, above < k ? g : 0xffffffffu);
+    if ((tid & 31) == 0) atomicMin(&sh.threshold, least);
   }
   __syncthreads();
   uint32_t limit = sh.threshold;
   if (!nan) {
+    // Vectors that reach the bound are set aside whole; then all threads look through their elements.
     const float bound = key_value(limit);
     if (thread_max >= bound || part.tiles > 1) {
-      // no barrier inside: threads below the bound pass over their vectors
       for (int tile = 0; tile < part.tiles; ++tile) {
         if (part.tiles > 1) part.load(tile);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          if (Vec16<T>::max(part.v[i]) >= bound)
-            part.elements(part.v[i], part.first(tile, i) + tid, [&](float x, int id) {
-              if (x >= bound) {
-                const int at = atomicAdd(&sh.n, 1);
-                if (at < kCandidates) sh.candidate[at] = entry_key(x, (uint32_t)id);
-              }
-            });
+          const int j = part.first(tile, i) + tid;
+          if (Vec16<T>::reaches(Vec16<T>::max_of(part.v[i]), bound) && j < part.j1) {
+            const int at = atomicAdd(&sh.hits, 1);
+            if (at < kHits) {
+              sh.hit[at] = part.v[i];
+              sh.hit_at[at] = j;
+            }
+          }
         }
       }
     }
     __syncthreads();
-    if (sh.n <= kCandidates) return sh.n;
+    if (sh.hits <= kHits) {
+      constexpr int kVec = Vec16<T>::kVec;
+      const int n = sh.hits * kVec;
+      for (int c = tid; c < n; c += NT) {
+        const float x = to_f32(reinterpret_cast<const T*>(sh.hit)[c]);
+        const int u = sh.hit_at[c / kVec] * kVec + c % kVec;
+        if (x >= bound && u >= part.row.lead && u < part.row.end) {
+          const int at = atomicAdd(&sh.n, 1);
+          if (at < kCandidates) sh.candidate[at] = entry_key(x, (uint32_t)(u - part.row.lead));
+        }
+      }
+      __syncthreads();
+      if (sh.n <= kCandidates) return sh.n;
+    }
+    __syncthreads();
   }
   // count the entries of the part with a key of at least `from`
   auto count = [&](uint32_t from) {
@@ -201,6 +227,7 @@ __device__ __forceinline__ int best_entries(Part<T, NT, N>& part, float thread_m
 // One CTA, or a cluster of them, for a row.
 template <typename T, int NT, int N, bool kTop>
 __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const dwarf_token_logprobs_args a, int cluster) {
+  using V = Vec16<T>;
   constexpr int kWarps = NT / 32;
   __shared__ Sums s_warp[kWarps];
   __shared__ float s_parts[kMaxCluster][3];
@@ -221,9 +248,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const dwa
   float thread_max = -CUDART_INF_F;
   for (int tile = 0; tile < part.tiles; ++tile) {
     part.load(tile);
-    float mx = Vec16<T>::max(part.v[0]);
+    typename V::Max mv = V::max_of(part.v[0]);
 #pragma unroll
-    for (int i = 1; i < N; ++i) mx = fmaxf(mx, Vec16<T>::max(part.v[i]));
+    for (int i = 1; i < N; ++i) mv = V::join(mv, V::max_of(part.v[i]));
+    const float mx = V::largest(mv);
     thread_max = fmaxf(thread_max, mx);
     const float m = fmaxf(sum.m, warp_max(mx));
     if (sum.m > -CUDART_INF_F) {  // a later tile: move the sums to the new maximum
@@ -234,18 +262,31 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const dwa
     sum.m = m;
     const float shift = m == -CUDART_INF_F ? 0.0f : -m;
     float2 s = make_float2(0.0f, 0.0f), t = s;
+    // Entries 2^-200 below the maximum count as 0, masked ones among them (0 (-inf) is
+    // not formed). The bound is set in the row's type where that has room for it below
+    // the maximum (2^-60 at least), in fp32 otherwise.
+    const typename V::Low low = V::low_of(m - 200.0f / c2);
+    const bool packed = (m - V::low_value(low)) * c2 >= 60.0f && V::low_value(low) > -1.0e38f;
+    auto add = [&](const uint4& w, bool clamp) {
+      float2 e[V::kVec / 2];
+      V::unpack(w, e);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (part.first(tile, i) >= part.j1) break;
-      float2 e[Part<T, NT, N>::kVec / 2];
-      Vec16<T>::unpack(part.v[i], e);
-#pragma unroll
-      for (int h = 0; h < Part<T, NT, N>::kVec / 2; ++h) {
-        const float2 d = mul2(add2(e[h], make_float2(shift, shift)), make_float2(c2, c2));
+      for (int h = 0; h < V::kVec / 2; ++h) {
+        float2 d = mul2(add2(e[h], make_float2(shift, shift)), make_float2(c2, c2));
         const float2 p = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+        if (clamp) d = make_float2(fmaxf(d.x, -200.0f), fmaxf(d.y, -200.0f));
         s = add2(s, p);
-        t = fma2(p, make_float2(fmaxf(d.x, -200.0f), fmaxf(d.y, -200.0f)), t);  // 0 (-inf) counts as 0
+        t = fma2(p, d, t);
       }
+    };
+    if (packed) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (part.first(tile, i) < part.j1) add(V::clamp(part.v[i], low), false);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (part.first(tile, i) < part.j1) add(part.v[i], true);
     }
     sum.s += s.x + s.y;
     sum.t += t.x + t.y;

@@ -105,9 +105,25 @@ struct Vec16<float> {
     return make_uint4(__float_as_uint(x[0].x), __float_as_uint(x[0].y), __float_as_uint(x[1].x),
                       __float_as_uint(x[1].y));
   }
-  // Largest element; NaN is passed over.
-  __device__ __forceinline__ static float max(const uint4& v) {
+  // A running maximum of elements by place (NaN is passed over), its largest, and whether one reaches `bound`.
+  using Max = float;
+  __device__ __forceinline__ static Max max_of(const uint4& v) {
     return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+  __device__ __forceinline__ static Max join(Max a, Max b) { return fmaxf(a, b); }
+  __device__ __forceinline__ static float largest(Max a) { return a; }
+  __device__ __forceinline__ static bool reaches(Max a, float bound) { return a >= bound; }
+  // Elements no lower than `low`.
+  using Low = float;
+  __device__ __forceinline__ static Low low_of(float v) { return v; }
+  __device__ __forceinline__ static float low_value(Low low) { return low; }
+  __device__ __forceinline__ static uint4 clamp(const uint4& v, Low low) {
+    return make_uint4(max_nan(v.x, low), max_nan(v.y, low), max_nan(v.z, low), max_nan(v.w, low));
+  }
+  __device__ __forceinline__ static uint32_t max_nan(uint32_t a, float b) {
+    uint32_t r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "f"(b));
+    return r;
   }
 };
 
@@ -129,10 +145,27 @@ struct Vec16<__nv_bfloat16> {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  __device__ __forceinline__ static float max(const uint4& v) {
+  using Max = __nv_bfloat162;
+  __device__ __forceinline__ static Max max_of(const uint4& v) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-    const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  }
+  __device__ __forceinline__ static Max join(Max a, Max b) { return __hmax2(a, b); }
+  __device__ __forceinline__ static float largest(Max a) {
+    const float2 f = __bfloat1622float2(a);
     return fmaxf(f.x, f.y);
+  }
+  __device__ __forceinline__ static bool reaches(Max a, float bound) { return largest(a) >= bound; }
+  using Low = __nv_bfloat162;
+  __device__ __forceinline__ static Low low_of(float v) { return __float2bfloat162_rn(v); }
+  __device__ __forceinline__ static float low_value(Low low) { return __low2float(low); }
+  __device__ __forceinline__ static uint4 clamp(const uint4& v, Low low) {
+    uint4 r;
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __hmax2_nan(h[i], low);
+    return r;
   }
 };
 
@@ -154,10 +187,27 @@ struct Vec16<__half> {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-  __device__ __forceinline__ static float max(const uint4& v) {
+  using Max = __half2;
+  __device__ __forceinline__ static Max max_of(const uint4& v) {
     const __half2* h = reinterpret_cast<const __half2*>(&v);
-    const float2 f = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  }
+  __device__ __forceinline__ static Max join(Max a, Max b) { return __hmax2(a, b); }
+  __device__ __forceinline__ static float largest(Max a) {
+    const float2 f = __half22float2(a);
     return fmaxf(f.x, f.y);
+  }
+  __device__ __forceinline__ static bool reaches(Max a, float bound) { return largest(a) >= bound; }
+  using Low = __half2;
+  __device__ __forceinline__ static Low low_of(float v) { return __float2half2_rn(v); }
+  __device__ __forceinline__ static float low_value(Low low) { return __low2float(low); }
+  __device__ __forceinline__ static uint4 clamp(const uint4& v, Low low) {
+    uint4 r;
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    __half2* o = reinterpret_cast<__half2*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __hmax2_nan(h[i], low);
+    return r;
   }
 };
 
