@@ -10,10 +10,12 @@
 namespace dwarf {
 namespace {
 
-constexpr int kVectors = 8;         // 16-byte vectors of a row that a thread holds
-constexpr int kCandidates = 512;    // entries that the search for the alternatives may sort
-constexpr int kHits = 512;          // vectors that it may look through
+constexpr int kRowThreads = 128;    // threads of a CTA of the forward kernel
+constexpr int kVectors = 8;         // 16-byte vectors of a row that a thread has in flight
 constexpr int kMaxCluster = 8;
+constexpr int kGroups = 2 * kRowThreads;
+constexpr int kCandidates = 512;    // entries that the search for the alternatives sorts
+constexpr int kHits = 512;          // vectors that it looks through
 
 // What a softmax needs of a part of a row: the maximum, S and T relative to it.
 struct Sums {
@@ -24,49 +26,36 @@ struct Sums {
 __device__ __forceinline__ Sums warp_join(Sums p, float c2) {
   const float m = warp_max(p.m);
   const float d = fmaxf((p.m - (m == -CUDART_INF_F ? 0.0f : m)) * c2, -200.0f);
-  const float f = p.s == 0.0f ? 0.0f : ex2_approx(d);
-  return {m, warp_sum(f * p.s), warp_sum(f * fmaf(d, p.s, p.t))};
+  const float f = ex2_approx(d);
+  return {m, warp_sum(p.s == 0.0f ? 0.0f : f * p.s), warp_sum(p.s == 0.0f ? 0.0f : f * fmaf(d, p.s, p.t))};
 }
 
-// The vectors of one row's part, NT threads and N vectors a thread at a time. A part
-// of one tile stays in registers; a longer one is read again by each walk.
-template <typename T, int NT, int N>
+// A CTA's part of a row, a tile of kVectors vectors for each thread at a time.
+template <typename T>
 struct Part {
   static constexpr int kVec = Vec16<T>::kVec;
   RowVectors<T> row;
-  int j0, j1, tiles;
-  uint4 v[N];
+  int j0, j1;  // the part's vectors
 
   __device__ __forceinline__ Part(const T* x, int vocab, int rank, int cluster) : row(x, vocab) {
     const int n = row.count(), per = ceil_div(n, cluster);
-    j0 = rank * per;
-    j1 = j0 + per < n ? j0 + per : n;
-    tiles = j1 > j0 ? ceil_div(j1 - j0, NT * N) : 0;
+    j0 = min(rank * per, n);
+    j1 = min(j0 + per, n);
   }
-  __device__ __forceinline__ int first(int tile, int i) const { return j0 + (tile * N + i) * NT; }
-  __device__ __forceinline__ void load(int tile) {
-    const int j = first(tile, 0) + threadIdx.x;
+  // Vectors first, first + threads, ...; places outside the part as -inf.
+  __device__ __forceinline__ void load(int first, uint4 (&v)[kVectors]) const {
+    const int j = first + threadIdx.x;
     const int lo = row.lead > 0 ? 1 : 0, hi = row.end / kVec;  // the whole vectors
     const uint4* p = reinterpret_cast<const uint4*>(row.base) + j;
-    if (first(tile, 0) >= lo && first(tile, N) <= (j1 < hi ? j1 : hi)) {
+    if (first >= lo && first + kVectors * kRowThreads <= min(j1, hi)) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = ld_stream(p + i * NT);
+      for (int i = 0; i < kVectors; ++i) v[i] = ld_stream(p + i * kRowThreads);
       return;
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < kVectors; ++i) {
       v[i] = make_uint4(Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf);
-      if (first(tile, i) < j1 && j + i * NT < j1) v[i] = row.load(j + i * NT);
-    }
-  }
-  // f(vector, j) in rising j; every thread of the block takes part in every step.
-  template <typename F>
-  __device__ __forceinline__ void walk(F f) {
-    for (int tile = 0; tile < tiles; ++tile) {
-      if (tiles > 1) load(tile);
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (first(tile, i) < j1) f(v[i], first(tile, i) + (int)threadIdx.x);
+      if (j + i * kRowThreads < j1) v[i] = row.load(j + i * kRowThreads);
     }
   }
   // f(value, id) for the elements of vector j that are in the row.
@@ -74,11 +63,20 @@ struct Part {
   __device__ __forceinline__ void elements(const uint4& w, int j, F f) const {
     float2 x[kVec / 2];
     Vec16<T>::unpack(w, x);
-    if (j >= j1) return;
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
       const int u = j * kVec + e;
       if (u >= row.lead && u < row.end) f(e & 1 ? x[e / 2].y : x[e / 2].x, u - row.lead);
+    }
+  }
+  // f(vector, j, whether j is in the part), one step of the whole block after the other, in rising j.
+  template <typename F>
+  __device__ __forceinline__ void walk(F f) const {
+    for (int first = j0; first < j1; first += kRowThreads) {
+      const int j = first + threadIdx.x;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (j < j1) w = row.load(j);
+      f(w, j, j < j1);
     }
   }
 };
@@ -88,116 +86,125 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 
 struct TopShared {
-  uint32_t value[512];               // order keys of the threads' maxima
-  uint32_t group[256];
-  uint4 hit[kHits];                  // vectors with an entry of at least the threshold
-  int hit_at[kHits];
+  uint32_t value[kGroups];           // order keys of the maxima, two of each thread
+  int hit[kHits];                    // vectors that reach the bound
   uint64_t candidate[kCandidates];
-  uint32_t threshold;
+  uint32_t bound;
   int n, hits;
-  int scan[16];
+  int scan[kRowThreads / 32];
 };
 
-// The K best entries of the part (order: value, then lowest id) among the first n
-// candidates, n >= min(K, entries of the part). The common case: with G >= 2 K groups
-// of threads, the K-th largest of the groups' maxima bounds the K-th entry from below,
-// and the entries from there up are few (G ln(G / (G - K)) if their places are random).
-// Where they are more than the buffer holds (ties, one group with many large values), or a
-// NaN is in the row, the K-th value is found bit by bit and its ties are taken in order.
-template <typename T, int NT, int N>
-__device__ __forceinline__ int best_entries(Part<T, NT, N>& part, float thread_max, int k, bool nan, TopShared& sh) {
-  const int tid = threadIdx.x;
-  int groups = 32;
-  while (groups < 2 * k && groups < NT && groups < 256) groups *= 2;
-  // sh.value was written before the caller's barrier
-  if (tid < groups) {
-    uint32_t g = 0;
-    for (int i = tid; i < NT; i += groups) g = max(g, sh.value[i]);
-    sh.group[tid] = g;
-  }
-  if (tid == 0) sh.n = sh.hits = 0, sh.threshold = 0xffffffffu;
-  __syncthreads();
-  if (tid < groups) {
-    // the K-th largest is the smallest that fewer than K exceed
-    const uint32_t g = sh.group[tid];
-    int above = 0;
-    const uint4* q = reinterpret_cast<const uint4*>(sh.group);
-    for (int i = 0; i < groups / 4; ++i) {
-      const uint4 w = q[i];
-      above += (w.x > g) + (w.y > g) + (w.z > g) + (w.w > g);
-    }
-    const uint32_t least = __reduce_min_sync(0xffffffffu, above < k ? g : 0xffffffffu);
-    if ((tid & 31) == 0) atomicMin(&sh.threshold, least);
-  }
-  __syncthreads();
-  uint32_t limit = sh.threshold;
-  if (!nan) {
-    // Vectors that reach the bound are set aside whole; then all threads look through their elements.
-    const float bound = key_value(limit);
-    if (thread_max >= bound || part.tiles > 1) {
-      for (int tile = 0; tile < part.tiles; ++tile) {
-        if (part.tiles > 1) part.load(tile);
+// A bound that K entries of the part reach: the smallest of the group maxima that the
+// K-th largest 16-bit prefix among them takes in. With G >= 2 K groups and entries in random
+// places about G ln(G / (G - K)) entries reach it. One warp searches the prefix bit by bit
+// (a rank of each group by comparison with all others took five times the instructions).
+__device__ __forceinline__ uint32_t bound_of_groups(const uint32_t* value, int k) {
+  const int lane = threadIdx.x & 31;
+  uint32_t g[kGroups / 32];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int j = part.first(tile, i) + tid;
-          if (Vec16<T>::reaches(Vec16<T>::max_of(part.v[i]), bound) && j < part.j1) {
-            const int at = atomicAdd(&sh.hits, 1);
-            if (at < kHits) {
-              sh.hit[at] = part.v[i];
-              sh.hit_at[at] = j;
-            }
-          }
+  for (int i = 0; i < kGroups / 32; ++i) g[i] = value[lane + 32 * i];
+  int groups = kGroups;
+#pragma unroll
+  for (int half = kGroups / 64; half >= 1; half /= 2) {
+    if (groups < 4 * k) break;
+    groups /= 2;
+#pragma unroll
+    for (int i = 0; i < half; ++i) g[i] = max(g[i], g[i + half]), g[i + half] = 0;
+  }
+  uint32_t prefix = 0;
+#pragma unroll
+  for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < kGroups / 32; ++i) c += g[i] >= (prefix | bit);
+    if (__reduce_add_sync(0xffffffffu, c) >= k) prefix |= bit;
+  }
+  uint32_t least = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < kGroups / 32; ++i)
+    if (g[i] >= prefix && g[i] > 0) least = min(least, g[i]);
+  return __reduce_min_sync(0xffffffffu, least);
+}
+
+// The K best entries of the part (order: value, then lowest id) among the first n
+// candidates, n >= min(K, entries of the part). `largest` holds 16 bits for each vector that are no
+// lower than its largest entry. The vectors that reach the bound are read again (from
+// L2) and their entries that reach it become candidates. Where these are more than the
+// buffers hold (ties, or many large values in one group), or a NaN is in the row, the
+// K-th value is found bit by bit over the whole part and its ties are taken in order.
+template <typename T>
+__device__ __forceinline__ int best_entries(const Part<T>& part, const typename Vec16<T>::Narrow* largest, int k,
+                                            bool nan, TopShared& sh) {
+  using N16 = Vec16<typename Vec16<T>::Narrow>;
+  const int tid = threadIdx.x;
+  uint32_t limit = sh.bound;
+  if (!nan) {
+    const float bound = key_value(limit);
+    const int n = part.j1 - part.j0;
+    for (int c = 8 * tid; c < n; c += 8 * kRowThreads) {
+      const uint4 w = *reinterpret_cast<const uint4*>(largest + c);
+      if (!N16::reaches(N16::max_of(w), bound)) continue;
+      const typename Vec16<T>::Narrow* e = reinterpret_cast<const typename Vec16<T>::Narrow*>(&w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (c + i < n && to_f32(e[i]) >= bound) {
+          const int at = atomicAdd(&sh.hits, 1);
+          if (at < kHits) sh.hit[at] = part.j0 + c + i;
         }
       }
     }
     __syncthreads();
-    if (sh.hits <= kHits) {
-      constexpr int kVec = Vec16<T>::kVec;
-      const int n = sh.hits * kVec;
-      for (int c = tid; c < n; c += NT) {
-        const float x = to_f32(reinterpret_cast<const T*>(sh.hit)[c]);
-        const int u = sh.hit_at[c / kVec] * kVec + c % kVec;
-        if (x >= bound && u >= part.row.lead && u < part.row.end) {
-          const int at = atomicAdd(&sh.n, 1);
-          if (at < kCandidates) sh.candidate[at] = entry_key(x, (uint32_t)(u - part.row.lead));
-        }
+    const int hits = sh.hits;
+    if (hits <= kHits) {
+      for (int h = tid; h < hits; h += kRowThreads) {
+        const int j = sh.hit[h];
+        part.elements(part.row.load(j), j, [&](float x, int id) {
+          if (x >= bound) {
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < kCandidates) sh.candidate[at] = entry_key(x, (uint32_t)id);
+          }
+        });
       }
       __syncthreads();
       if (sh.n <= kCandidates) return sh.n;
     }
     __syncthreads();
   }
-  // count the entries of the part with a key of at least `from`
+  // entries of the part with a key of at least `from`
   auto count = [&](uint32_t from) {
     int c = 0;
-    part.walk([&](const uint4& w, int j) { part.elements(w, j, [&](float x, int) { c += order_key(x) >= from; }); });
+    part.walk([&](const uint4& w, int j, bool in) {
+      if (in) part.elements(w, j, [&](float x, int) { c += order_key(x) >= from; });
+    });
     c = __reduce_add_sync(0xffffffffu, c);
     __syncthreads();
     if ((tid & 31) == 0) sh.scan[tid >> 5] = c;
     __syncthreads();
     c = 0;
-    for (int i = 0; i < NT / 32; ++i) c += sh.scan[i];
+#pragma unroll
+    for (int i = 0; i < kRowThreads / 32; ++i) c += sh.scan[i];
     return c;
   };
   if (nan || count(limit + 1) >= k) {
     limit = 0;
-    for (int bit = 31; bit >= 0; --bit)
-      if (count(limit | (1u << bit)) >= k) limit |= 1u << bit;
+    for (uint32_t bit = 0x80000000u; bit != 0; bit >>= 1)
+      if (count(limit | bit) >= k) limit |= bit;
   }
   __syncthreads();
   if (tid == 0) sh.n = 0;
   __syncthreads();
-  part.walk([&](const uint4& w, int j) {
-    part.elements(w, j, [&](float x, int id) {
-      if (order_key(x) > limit) sh.candidate[atomicAdd(&sh.n, 1)] = entry_key(x, (uint32_t)id);  // fewer than k
-    });
+  part.walk([&](const uint4& w, int j, bool in) {
+    if (in)
+      part.elements(w, j, [&](float x, int id) {
+        if (order_key(x) > limit) sh.candidate[atomicAdd(&sh.n, 1)] = entry_key(x, (uint32_t)id);  // fewer than k
+      });
   });
   __syncthreads();
   int have = sh.n;
-  part.walk([&](const uint4& w, int j) {
+  part.walk([&](const uint4& w, int j, bool in) {
     if (have >= k) return;  // the same for the whole block
     int c = 0;
-    part.elements(w, j, [&](float x, int) { c += order_key(x) == limit; });
+    if (in) part.elements(w, j, [&](float x, int) { c += order_key(x) == limit; });
     int at = c;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -207,16 +214,18 @@ __device__ __forceinline__ int best_entries(Part<T, NT, N>& part, float thread_m
     if ((tid & 31) == 31) sh.scan[tid >> 5] = at;
     __syncthreads();
     int total = 0;
-    for (int i = 0; i < NT / 32; ++i) {
+#pragma unroll
+    for (int i = 0; i < kRowThreads / 32; ++i) {
       if (i < (tid >> 5)) at += sh.scan[i];
       total += sh.scan[i];
     }
     at += have - c;
-    part.elements(w, j, [&](float x, int id) {
-      if (order_key(x) != limit) return;
-      if (at < k) sh.candidate[at] = entry_key(x, (uint32_t)id);
-      ++at;
-    });
+    if (in)
+      part.elements(w, j, [&](float x, int id) {
+        if (order_key(x) != limit) return;
+        if (at < k) sh.candidate[at] = entry_key(x, (uint32_t)id);
+        ++at;
+      });
     have = min(k, have + total);
     __syncthreads();
   });
@@ -224,15 +233,21 @@ __device__ __forceinline__ int best_entries(Part<T, NT, N>& part, float thread_m
   return have;
 }
 
-// One CTA, or a cluster of them, for a row.
-template <typename T, int NT, int N, bool kTop>
-__global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const dwarf_token_logprobs_args a, int cluster) {
+// One CTA, or a cluster of them, for a row: one pass that keeps a running maximum, S
+// and T for each warp. Eight CTAs of 128 threads on an SM overlap one's loads with
+// another's sums and search; 512 threads that hold a whole row reached 4.0 of these
+// 6.4 TB/s (16384 rows of 32768 bf16, no alternatives).
+template <typename T, bool kTop>
+__global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
+    token_logprobs_kernel(const dwarf_token_logprobs_args a, int cluster, int lists_at) {
   using V = Vec16<T>;
-  constexpr int kWarps = NT / 32;
+  constexpr int kWarps = kRowThreads / 32;
+  extern __shared__ __align__(16) unsigned char s_dynamic[];
+  typename V::Narrow* s_largest = reinterpret_cast<typename V::Narrow*>(s_dynamic);
+  uint64_t* s_lists = reinterpret_cast<uint64_t*>(s_dynamic + lists_at);  // [cluster][k], in rank 0
   __shared__ Sums s_warp[kWarps];
   __shared__ float s_parts[kMaxCluster][3];
   __shared__ Sums s_row;
-  __shared__ uint64_t s_lists[kTop ? kMaxCluster * DWARF_TOP_K_MAX : 1];
   __shared__ __align__(16) unsigned char s_top[kTop ? sizeof(TopShared) : 16];
   TopShared& top = *reinterpret_cast<TopShared*>(s_top);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -243,16 +258,25 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const dwa
   const float c2 = a.inv_temperature * kLog2e;
   if (cluster > 1) cluster_arrive();  // its CTAs have started, before one writes to another
 
-  Part<T, NT, N> part(x, vocab, rank, cluster);
+  const Part<T> part(x, vocab, rank, cluster);
   Sums sum = {-CUDART_INF_F, 0.0f, 0.0f};
-  float thread_max = -CUDART_INF_F;
-  for (int tile = 0; tile < part.tiles; ++tile) {
-    part.load(tile);
-    typename V::Max mv = V::max_of(part.v[0]);
+  float top0 = -CUDART_INF_F, top1 = -CUDART_INF_F;  // maxima of the thread's even and odd vectors
+  for (int first = part.j0; first < part.j1; first += kVectors * kRowThreads) {
+    uint4 v[kVectors];
+    part.load(first, v);
+    typename V::Max mv[2];
 #pragma unroll
-    for (int i = 1; i < N; ++i) mv = V::join(mv, V::max_of(part.v[i]));
-    const float mx = V::largest(mv);
-    thread_max = fmaxf(thread_max, mx);
+    for (int i = 0; i < kVectors; ++i) {
+      const typename V::Max of = V::max_of(v[i]);
+      mv[i & 1] = i < 2 ? of : V::join(mv[i & 1], of);
+      const int j = first - part.j0 + i * kRowThreads + tid;
+      if (kTop && j < part.j1 - part.j0) s_largest[j] = V::narrow(of);
+    }
+    const float mx = V::largest(V::join(mv[0], mv[1]));
+    if (kTop) {
+      top0 = fmaxf(top0, V::largest(mv[0]));
+      top1 = fmaxf(top1, V::largest(mv[1]));
+    }
     const float m = fmaxf(sum.m, warp_max(mx));
     if (sum.m > -CUDART_INF_F) {  // a later tile: move the sums to the new maximum
       const float d = fmaxf((sum.m - m) * c2, -200.0f), f = ex2_approx(d);
@@ -281,12 +305,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const dwa
     };
     if (packed) {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (part.first(tile, i) < part.j1) add(V::clamp(part.v[i], low), false);
+      for (int i = 0; i < kVectors; ++i)
+        if (first + i * kRowThreads < part.j1) add(V::clamp(v[i], low), false);
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (part.first(tile, i) < part.j1) add(part.v[i], true);
+      for (int i = 0; i < kVectors; ++i)
+        if (first + i * kRowThreads < part.j1) add(v[i], true);
     }
     sum.s += s.x + s.y;
     sum.t += t.x + t.y;
@@ -294,7 +318,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const dwa
   sum.s = warp_sum(sum.s);
   sum.t = warp_sum(sum.t);
   if (lane == 0) s_warp[warp] = sum;
-  if (kTop) top.value[tid] = order_key(thread_max);
+  if (kTop) {
+    top.value[tid] = order_key(top0);
+    top.value[kRowThreads + tid] = order_key(top1);
+    if (tid == 0) top.n = top.hits = 0;
+  }
   __syncthreads();
   if (cluster > 1) cluster_wait();
   if (!kTop && warp != kWarps - 1 && cluster == 1) return;
@@ -309,14 +337,20 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const dwa
   }
   int n = 0;
   if (kTop) {
+    if (warp == 0) {
+      const uint32_t bound = bound_of_groups(top.value, k);
+      if (lane == 0) top.bound = bound;
+    }
+    __syncthreads();
     // a NaN or +inf anywhere in the part makes some warp's sum NaN
     bool nan = false;
+#pragma unroll
     for (int w = 0; w < kWarps; ++w) nan |= s_warp[w].s != s_warp[w].s;
-    n = best_entries(part, thread_max, k, nan, top);
+    n = best_entries(part, s_largest, k, nan, top);
   }
   if (cluster > 1) {
     if (kTop) {
-      for (int c = tid; c < max(n, k); c += NT) {
+      for (int c = tid; c < max(n, k); c += kRowThreads) {
         uint64_t key = 0;
         int at = c;
         if (c < n) {
@@ -366,14 +400,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const dwa
         fin.s == 0.0f ? -CUDART_INF_F : (key_value((uint32_t)(key >> 32)) - fin.m) * a.inv_temperature - fin.t;
   };
   if (cluster == 1) {
-    for (int c = tid; c < n; c += NT) {
+    for (int c = tid; c < n; c += kRowThreads) {
       const uint64_t key = top.candidate[c];
       int at = 0;
       for (int i = 0; i < n; ++i) at += top.candidate[i] > key;
       if (at < k) put(key, at);
     }
   } else {
-    for (int c = tid; c < cluster * k; c += NT) {
+    for (int c = tid; c < cluster * k; c += kRowThreads) {
       const uint64_t key = s_lists[c];
       if (key == 0) continue;  // a part with fewer than k entries
       int at = c % k;
@@ -391,12 +425,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const dwa
   }
 }
 
-// How many CTAs share a row: enough that its part fits a CTA's registers, and more
-// while the rows alone leave SMs without work and a part keeps 128 vectors or more.
-inline int cluster_for(int64_t rows, int vectors, int tile) {
+// How many CTAs share a row: more than one only while the rows alone leave SMs with
+// fewer than four CTAs and each part keeps a vector for every thread (148 rows of 32768 bf16:
+// 12.3 us with one CTA each, 11.1 with four; 1000 rows: 22.1 with one, 23.3 with two),
+// or where a part's vector maxima would take over 64 KB of shared memory.
+inline int cluster_for(int64_t rows, int vectors) {
   int c = 1;
-  while (c < kMaxCluster && vectors > c * tile) c *= 2;
-  while (c < kMaxCluster && rows * c * 2 <= kNumSMs && vectors >= c * 2 * 128) c *= 2;
+  while (c < kMaxCluster && vectors > c * 32768) c *= 2;
+  while (c < kMaxCluster && rows * c * 2 <= 4 * kNumSMs && vectors >= c * 2 * kRowThreads) c *= 2;
   return c;
 }
 
@@ -404,15 +440,17 @@ template <typename T>
 int launch_forward(const dwarf_token_logprobs_args& a, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner;
   const int vectors = ceil_div((int)a.vocab, Vec16<T>::kVec);
-  const int cluster = cluster_for(rows, vectors, 512 * kVectors);
-  const int part = ceil_div(vectors, cluster);
-  // 128 threads where they hold the part and the groups that bound the alternatives
-  const bool small = part <= 128 * kVectors && a.top_k <= 32;
-  if (a.top_k > 0)
-    return small ? launch_rows(token_logprobs_kernel<T, 128, kVectors, true>, rows, cluster, 128, 0, stream, a, cluster)
-                 : launch_rows(token_logprobs_kernel<T, 512, kVectors, true>, rows, cluster, 512, 0, stream, a, cluster);
-  return small ? launch_rows(token_logprobs_kernel<T, 128, kVectors, false>, rows, cluster, 128, 0, stream, a, cluster)
-               : launch_rows(token_logprobs_kernel<T, 512, kVectors, false>, rows, cluster, 512, 0, stream, a, cluster);
+  const int cluster = cluster_for(rows, vectors);
+  if (a.top_k == 0)
+    return launch_rows(token_logprobs_kernel<T, false>, rows, cluster, kRowThreads, 0, stream, a, cluster, 0);
+  // a row that starts off a 16-byte boundary has one vector more
+  const int lists_at = (ceil_div(vectors + 1, cluster) * 2 + 15) / 16 * 16;
+  const int bytes = lists_at + (cluster > 1 ? cluster * a.top_k * 8 : 0);
+  const auto kernel = token_logprobs_kernel<T, true>;
+  if (bytes > 32 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return launch_status();
+  return launch_rows(kernel, rows, cluster, kRowThreads, bytes, stream, a, cluster, lists_at);
 }
 
 constexpr int kThreads = 256;

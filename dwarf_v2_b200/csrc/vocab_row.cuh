@@ -112,6 +112,8 @@ struct Vec16<float> {
   }
   __device__ __forceinline__ static Max join(Max a, Max b) { return fmaxf(a, b); }
   __device__ __forceinline__ static float largest(Max a) { return a; }
+  using Narrow = __nv_bfloat16;  // 16 bits that are no lower than the largest
+  __device__ __forceinline__ static Narrow narrow(Max a) { return __float2bfloat16_ru(a); }
   __device__ __forceinline__ static bool reaches(Max a, float bound) { return a >= bound; }
   // Elements no lower than `low`.
   using Low = float;
@@ -146,6 +148,8 @@ struct Vec16<__nv_bfloat16> {
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
   using Max = __nv_bfloat162;
+  using Narrow = __nv_bfloat16;
+  __device__ __forceinline__ static Narrow narrow(Max a) { return __hmax(__low2bfloat16(a), __high2bfloat16(a)); }
   __device__ __forceinline__ static Max max_of(const uint4& v) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
     return __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
@@ -188,6 +192,8 @@ struct Vec16<__half> {
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
   using Max = __half2;
+  using Narrow = __half;
+  __device__ __forceinline__ static Narrow narrow(Max a) { return __hmax(__low2half(a), __high2half(a)); }
   __device__ __forceinline__ static Max max_of(const uint4& v) {
     const __half2* h = reinterpret_cast<const __half2*>(&v);
     return __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
