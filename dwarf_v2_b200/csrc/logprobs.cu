@@ -10,9 +10,6 @@
 namespace dwarf {
 namespace {
 
-constexpr int kRowThreads = 128;    // threads of a CTA of the forward kernel
-constexpr int kVectors = 8;         // 16-byte vectors of a row that a thread has in flight
-constexpr int kMaxCluster = 8;
 constexpr int kGroups = 2 * kRowThreads;
 constexpr int kCandidates = 512;    // entries that the search for the alternatives sorts
 constexpr int kHits = 512;          // vectors that it looks through
@@ -29,57 +26,6 @@ __device__ __forceinline__ Sums warp_join(Sums p, float c2) {
   const float f = ex2_approx(d);
   return {m, warp_sum(p.s == 0.0f ? 0.0f : f * p.s), warp_sum(p.s == 0.0f ? 0.0f : f * fmaf(d, p.s, p.t))};
 }
-
-// A CTA's part of a row, a tile of kVectors vectors for each thread at a time.
-template <typename T>
-struct Part {
-  static constexpr int kVec = Vec16<T>::kVec;
-  RowVectors<T> row;
-  int j0, j1;  // the part's vectors
-
-  __device__ __forceinline__ Part(const T* x, int vocab, int rank, int cluster) : row(x, vocab) {
-    const int n = row.count(), per = ceil_div(n, cluster);
-    j0 = min(rank * per, n);
-    j1 = min(j0 + per, n);
-  }
-  // Vectors first, first + threads, ...; places outside the part as -inf.
-  __device__ __forceinline__ void load(int first, uint4 (&v)[kVectors]) const {
-    const int j = first + threadIdx.x;
-    const int lo = row.lead > 0 ? 1 : 0, hi = row.end / kVec;  // the whole vectors
-    const uint4* p = reinterpret_cast<const uint4*>(row.base) + j;
-    if (first >= lo && first + kVectors * kRowThreads <= min(j1, hi)) {
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i) v[i] = ld_stream(p + i * kRowThreads);
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      v[i] = make_uint4(Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf);
-      if (j + i * kRowThreads < j1) v[i] = row.load(j + i * kRowThreads);
-    }
-  }
-  // f(value, id) for the elements of vector j that are in the row.
-  template <typename F>
-  __device__ __forceinline__ void elements(const uint4& w, int j, F f) const {
-    float2 x[kVec / 2];
-    Vec16<T>::unpack(w, x);
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      const int u = j * kVec + e;
-      if (u >= row.lead && u < row.end) f(e & 1 ? x[e / 2].y : x[e / 2].x, u - row.lead);
-    }
-  }
-  // f(vector, j, whether j is in the part), one step of the whole block after the other, in rising j.
-  template <typename F>
-  __device__ __forceinline__ void walk(F f) const {
-    for (int first = j0; first < j1; first += kRowThreads) {
-      const int j = first + threadIdx.x;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (j < j1) w = row.load(j);
-      f(w, j, j < j1);
-    }
-  }
-};
 
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
@@ -425,22 +371,11 @@ __global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
   }
 }
 
-// How many CTAs share a row: more than one only while the rows alone leave SMs with
-// fewer than four CTAs and each part keeps a vector for every thread (148 rows of 32768 bf16:
-// 12.3 us with one CTA each, 11.1 with four; 1000 rows: 22.1 with one, 23.3 with two),
-// or where a part's vector maxima would take over 64 KB of shared memory.
-inline int cluster_for(int64_t rows, int vectors) {
-  int c = 1;
-  while (c < kMaxCluster && vectors > c * 32768) c *= 2;
-  while (c < kMaxCluster && rows * c * 2 <= 4 * kNumSMs && vectors >= c * 2 * kRowThreads) c *= 2;
-  return c;
-}
-
 template <typename T>
 int launch_forward(const dwarf_token_logprobs_args& a, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner;
   const int vectors = ceil_div((int)a.vocab, Vec16<T>::kVec);
-  const int cluster = cluster_for(rows, vectors);
+  const int cluster = cluster_for(rows, vectors, 32768);  // vector maxima: at most 64 KB
   if (a.top_k == 0)
     return launch_rows(token_logprobs_kernel<T, false>, rows, cluster, kRowThreads, 0, stream, a, cluster, 0);
   // a row that starts off a 16-byte boundary has one vector more
@@ -453,59 +388,90 @@ int launch_forward(const dwarf_token_logprobs_args& a, cudaStream_t stream) {
   return launch_rows(kernel, rows, cluster, kRowThreads, bytes, stream, a, cluster, lists_at);
 }
 
-constexpr int kThreads = 256;
-
+// grad_v = c (sparse terms - q_v (G + gH (log q_v + H))): each CTA writes its part of the
+// row, then the listed entries of that part again with their terms. One read of the
+// logits, one write; q from the forward's m and S.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(dwarf_token_logprobs_bwd_args a) {
-  __shared__ float sf[kThreads / 32];
-  __shared__ int64_t s_id[DWARF_TOP_K_MAX + 1];
+__global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
+    token_logprobs_bwd_kernel(const dwarf_token_logprobs_bwd_args a, int parts) {
+  using V = Vec16<T>;
+  __shared__ float sf[kRowThreads / 32];
+  __shared__ int s_id[DWARF_TOP_K_MAX + 1];
   __shared__ float s_g[DWARF_TOP_K_MAX + 1];
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(a.logits) + row_offset(row, a.inner, a.so, a.si);
-  T* out = static_cast<T*>(a.grad) + row * a.vocab;
+  const int tid = threadIdx.x;
+  const int64_t r = blockIdx.x / (unsigned)parts;
+  const T* x = static_cast<const T*>(a.logits) + row_offset(r, a.inner, a.so, a.si);
   const int vocab = (int)a.vocab;
+  const Part<T> part(x, vocab, blockIdx.x % (unsigned)parts, parts);
+  const RowStore<T> store(static_cast<T*>(a.grad) + r * a.vocab, part.row);
   const float c2 = a.inv_temperature * kLog2e;
-  const float2 ms = reinterpret_cast<const float2*>(a.stats)[row];
+  const float2 ms = reinterpret_cast<const float2*>(a.stats)[r];
   // entry 0: the target; entries 1..top_k: the alternatives
-  float g_lp = a.g_logprob != nullptr ? a.g_logprob[row] : 0.0f;
-  const int64_t target = a.targets != nullptr ? a.targets[row] : -1;
+  float g_lp = a.g_logprob != nullptr ? a.g_logprob[r] : 0.0f;
+  const int64_t target = a.targets != nullptr ? a.targets[r] : -1;
   if (a.targets == nullptr || target == a.ignore_index) g_lp = 0.0f;
   const bool off = g_lp != 0.0f && (target < 0 || target >= vocab);
   const int n = a.g_top != nullptr ? a.top_k + 1 : 1;
   float g = 0.0f;
   bool any = g_lp != 0.0f;
-  for (int j = threadIdx.x; j < n; j += kThreads) {
-    const float v = j == 0 ? g_lp : a.g_top[row * a.top_k + j - 1];
-    s_id[j] = j == 0 ? (g_lp != 0.0f && !off ? target : -1) : a.top_ids[row * a.top_k + j - 1];
+  for (int j = tid; j < n; j += kRowThreads) {
+    const float v = j == 0 ? g_lp : a.g_top[r * a.top_k + j - 1];
+    s_id[j] = j == 0 ? (g_lp != 0.0f && !off ? (int)target : -1) : (int)a.top_ids[r * a.top_k + j - 1];
     s_g[j] = v;
     g += v;
     any |= v != 0.0f;
   }
-  g = block_reduce<kThreads>(g, sf, AddOp());
-  const float g_lse = a.g_lse != nullptr ? a.g_lse[row] : 0.0f;
-  const float g_h = a.g_entropy != nullptr ? a.g_entropy[row] : 0.0f;
+  g = n > 1 ? block_reduce<kRowThreads>(g, sf, AddOp()) : g_lp;
+  const float g_lse = a.g_lse != nullptr ? a.g_lse[r] : 0.0f;
+  const float g_h = a.g_entropy != nullptr ? a.g_entropy[r] : 0.0f;
   any = __syncthreads_or(any) || g_lse != 0.0f || g_h != 0.0f;
   if (!any || ms.y == 0.0f) {
-    for (int i = threadIdx.x; i < vocab; i += kThreads) out[i] = from_f32<T>(0.0f);
+    for (int j = part.j0 + tid; j < part.j1; j += kRowThreads) store.zero(j);
     return;
   }
   const float weight = off ? CUDART_NAN_F : g - g_lse;
-  const float inv_s = 1.0f / ms.y, log2s = log2f(ms.y), h2 = a.entropy[row] * kLog2e - log2s;
-  auto dense = [&](float v) {
-    const float d = (v - ms.x) * c2;
-    const float q = ex2_approx(d) * inv_s;
-    return -q * (weight + g_h * kLn2 * (fmaxf(d, -200.0f) + h2));
+  const float log2s = log2f(ms.y), h2 = a.entropy[r] * kLog2e - log2s;
+  // -q c (G + gH ln2 (d + h2)) = e (A + B d)
+  const float scale = -a.inv_temperature / ms.y;
+  const float k_b = scale * g_h * kLn2, k_a = fmaf(k_b, h2, scale * weight);
+  const float2 shift = make_float2(-ms.x, -ms.x), cc = make_float2(c2, c2);
+  auto dense = [&](float2 v) {
+    float2 d = mul2(add2(v, shift), cc);
+    const float2 e = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+    d = make_float2(fmaxf(d.x, -200.0f), fmaxf(d.y, -200.0f));
+    return mul2(e, fma2(make_float2(k_b, k_b), d, make_float2(k_a, k_a)));
   };
-  for (int i = threadIdx.x; i < vocab; i += kThreads) out[i] = from_f32<T>(a.inv_temperature * dense(to_f32(x[i])));
+  for (int first = part.j0; first < part.j1; first += kVectors * kRowThreads) {
+    uint4 v[kVectors];
+    part.load(first, v);
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+      const int j = first + i * kRowThreads + tid;
+      if (j >= part.j1) break;
+      float2 e[V::kVec / 2];
+      V::unpack(v[i], e);
+#pragma unroll
+      for (int h = 0; h < V::kVec / 2; ++h) e[h] = dense(e[h]);
+      store.put(j, V::pack(e));
+    }
+  }
   __syncthreads();  // the listed entries are written again, with their own terms
-  for (int j = threadIdx.x; j < n; j += kThreads) {
-    const int64_t id = s_id[j];
-    if (id < 0 || id >= vocab) continue;
+  for (int j = tid; j < n; j += kRowThreads) {
+    const int id = s_id[j];
+    if (id < 0 || id >= vocab || !part.holds(id)) continue;
     float sum = 0.0f;
     for (int l = 0; l < n; ++l)
       if (s_id[l] == id) sum += s_g[l];
-    out[id] = from_f32<T>(a.inv_temperature * (sum + dense(to_f32(x[id]))));
+    const float v = to_f32(x[id]);
+    store.out[id] = from_f32<T>(fmaf(a.inv_temperature, sum, dense(make_float2(v, v)).x));
   }
+}
+
+template <typename T>
+int launch_backward(const dwarf_token_logprobs_bwd_args& a, cudaStream_t stream) {
+  const int64_t rows = a.outer * a.inner;
+  const int parts = parts_for(rows, ceil_div((int)a.vocab, Vec16<T>::kVec));
+  return launch_rows(token_logprobs_bwd_kernel<T>, rows * parts, 1, kRowThreads, 0, stream, a, parts);
 }
 
 template <typename F>
@@ -545,8 +511,5 @@ extern "C" int dwarf_token_logprobs_bwd(const dwarf_token_logprobs_bwd_args* arg
   if (a.stats == nullptr || a.entropy == nullptr || a.grad == nullptr) return DWARF_ERR_NULL;
   if (a.g_logprob != nullptr && a.targets == nullptr) return DWARF_ERR_NULL;
   if (a.g_top != nullptr && (a.top_ids == nullptr || a.top_k < 1)) return DWARF_ERR_NULL;
-  return with_type(a.dtype, [&](auto t) {
-    token_logprobs_bwd_kernel<decltype(t)><<<(unsigned)rows, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    return launch_status();
-  });
+  return with_type(a.dtype, [&](auto t) { return launch_backward<decltype(t)>(a, static_cast<cudaStream_t>(stream)); });
 }

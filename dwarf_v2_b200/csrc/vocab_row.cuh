@@ -10,6 +10,9 @@ namespace dwarf {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kRowThreads = 128;    // threads of a CTA, or of each CTA of a cluster, for a row
+constexpr int kVectors = 8;         // 16-byte vectors of a row that a thread has in flight
+constexpr int kMaxCluster = 8;
 
 // Row r of logits [outer, inner, vocab] with two row strides.
 __device__ __forceinline__ int64_t row_offset(int64_t r, int64_t inner, int64_t so, int64_t si) {
@@ -224,6 +227,11 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
   return v;
 }
 
+__device__ __forceinline__ void st_stream(void* p, const uint4& v) {
+  asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+
 // A row as aligned 16-byte vectors. Places u count from the 16-byte boundary at or
 // before the row's first element: element id lies at u = id + lead, vector j holds
 // places [j kVec, (j + 1) kVec). Only the first and the last vector may hold places
@@ -311,6 +319,105 @@ int launch_rows(void (*kernel)(Params...), int64_t rows, int cluster, int thread
   cfg.numAttrs = cluster > 1 ? 1 : 0;
   if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) return launch_status();
   return launch_status();
+}
+
+// A CTA's part of a row, a tile of kVectors vectors for each thread at a time.
+template <typename T>
+struct Part {
+  static constexpr int kVec = Vec16<T>::kVec;
+  RowVectors<T> row;
+  int j0, j1;  // the part's vectors
+
+  __device__ __forceinline__ Part(const T* x, int vocab, int rank, int cluster) : row(x, vocab) {
+    const int n = row.count(), per = ceil_div(n, cluster);
+    j0 = min(rank * per, n);
+    j1 = min(j0 + per, n);
+  }
+  // Vectors first, first + threads, ...; places outside the part as -inf.
+  __device__ __forceinline__ void load(int first, uint4 (&v)[kVectors]) const {
+    const int j = first + threadIdx.x;
+    const int lo = row.lead > 0 ? 1 : 0, hi = row.end / kVec;  // the whole vectors
+    const uint4* p = reinterpret_cast<const uint4*>(row.base) + j;
+    if (first >= lo && first + kVectors * kRowThreads <= min(j1, hi)) {
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) v[i] = ld_stream(p + i * kRowThreads);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+      v[i] = make_uint4(Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf);
+      if (j + i * kRowThreads < j1) v[i] = row.load(j + i * kRowThreads);
+    }
+  }
+  __device__ __forceinline__ bool holds(int id) const {
+    const int j = (id + row.lead) / kVec;
+    return j >= j0 && j < j1;
+  }
+  // f(value, id) for the elements of vector j that are in the row.
+  template <typename F>
+  __device__ __forceinline__ void elements(const uint4& w, int j, F f) const {
+    float2 x[kVec / 2];
+    Vec16<T>::unpack(w, x);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      const int u = j * kVec + e;
+      if (u >= row.lead && u < row.end) f(e & 1 ? x[e / 2].y : x[e / 2].x, u - row.lead);
+    }
+  }
+  // f(vector, j, whether j is in the part), one step of the whole block after the other, in rising j.
+  template <typename F>
+  __device__ __forceinline__ void walk(F f) const {
+    for (int first = j0; first < j1; first += kRowThreads) {
+      const int j = first + threadIdx.x;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (j < j1) w = row.load(j);
+      f(w, j, j < j1);
+    }
+  }
+};
+
+// Where the values of a row's vectors go: whole vectors at once where the output row lies
+// on the same 16-byte boundaries as the logits, else (a slice of an odd vocabulary) by element.
+template <typename T>
+struct RowStore {
+  static constexpr int kVec = Vec16<T>::kVec;
+  T* out;
+  const RowVectors<T>& row;
+  bool same;
+  __device__ __forceinline__ RowStore(T* o, const RowVectors<T>& r) : out(o), row(r) {
+    same = (reinterpret_cast<uintptr_t>(o) & 15) == r.lead * sizeof(T);
+  }
+  __device__ __forceinline__ void put(int j, const uint4& v) const {
+    if (same && row.whole(j)) {
+      st_stream(out + ((int64_t)j * kVec - row.lead), v);
+      return;
+    }
+    const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const int u = j * kVec + i;
+      if (u >= row.lead && u < row.end) out[u - row.lead] = e[i];
+    }
+  }
+  __device__ __forceinline__ void zero(int j) const { put(j, make_uint4(0, 0, 0, 0)); }
+};
+
+// How many CTAs share a row: more than one only while the rows alone leave SMs with
+// fewer than four CTAs and each part keeps a vector for every thread (148 rows of 32768 bf16:
+// 12.3 us with one CTA each, 11.1 with four; 1000 rows: 22.1 with one, 23.3 with two),
+// or where a part would have over `most` vectors.
+inline int cluster_for(int64_t rows, int vectors, int most) {
+  int c = 1;
+  while (c < kMaxCluster && vectors > c * most) c *= 2;
+  while (c < kMaxCluster && rows * c * 2 <= 4 * kNumSMs && vectors >= c * 2 * kRowThreads) c *= 2;
+  return c;
+}
+
+// The same where the CTAs of a row need nothing of each other.
+inline int parts_for(int64_t rows, int vectors) {
+  int c = 1;
+  while (rows * c * 2 <= 8 * kNumSMs && vectors >= c * 2 * kRowThreads) c *= 2;
+  return c;
 }
 
 // Host checks shared by the entry points: sizes, strides and the scale of a logit tensor.
