@@ -12,22 +12,33 @@
 namespace dwarf {
 namespace {
 
-static_assert(kRowThreads >= DWARF_TOP_K_MAX, "one thread for each slot of the teacher's list");
+// (m, sums relative to m) of a warp's lanes joined, in a fixed order; lanes without a part: m = -inf, sums 0.
+__device__ __forceinline__ void warp_join(float c2, float& m, float& a, float& b) {
+  const float top = warp_max(m);
+  const float f = ex2_approx((m - (top == -CUDART_INF_F ? 0.0f : top)) * c2);
+  m = top;
+  a = warp_sum(a == 0.0f ? 0.0f : f * a);
+  b = warp_sum(b == 0.0f ? 0.0f : f * b);
+}
 
-// Two passes over the row where the gradient is wanted, the second from L2 (the eight CTAs
-// of an SM hold 148 * 8 rows at a time: 77 MB of bf16 at a vocabulary of 32768).
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
-    topk_distill_kernel(const dwarf_topk_distill_args a, int cluster) {
+// kKeep: the part's vectors stay in shared memory between the sums and the gradient; every
+// thread reads back only what it copied there itself. Otherwise they are read again.
+template <typename T, int NT, bool kKeep>
+__global__ void __launch_bounds__(NT, (kKeep ? 768 : 1024) / NT)
+    topk_distill_kernel(const dwarf_topk_distill_args a, int cluster, int bits_at) {
   using V = Vec16<T>;
-  constexpr int kWarps = kRowThreads / 32;
-  extern __shared__ __align__(16) uint32_t listed[];  // a bit for each place of the part
-  __shared__ float s_m[kWarps], s_rest[kWarps], s_list[kWarps];
+  constexpr int kWarps = NT / 32;
+  static_assert(NT >= DWARF_TOP_K_MAX, "one thread for each slot of the teacher's list");
+  extern __shared__ __align__(16) unsigned char s_dynamic[];
+  uint4* s_kept = reinterpret_cast<uint4*>(s_dynamic);
+  uint32_t* listed = reinterpret_cast<uint32_t*>(s_dynamic + bits_at);  // a bit for each place of the part
+  __shared__ float s_m[kWarps], s_rest[kWarps], s_list[kWarps], s_term[kWarps];
+  __shared__ float s_top[kWarps];
+  __shared__ double s_sum[kWarps];
   __shared__ float s_parts[kMaxCluster][3];
-  __shared__ float sf[kWarps];
-  __shared__ double sd[kWarps];
   __shared__ int s_id[DWARF_TOP_K_MAX];
   __shared__ float s_p[DWARF_TOP_K_MAX];
+  __shared__ int s_flags, s_listed;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int vocab = (int)a.vocab, k = a.k;
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
@@ -40,65 +51,80 @@ __global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
   }
   if (cluster > 1) cluster_arrive();  // its CTAs have started, before one writes to another
   const T* x = static_cast<const T*>(a.logits) + row_offset(r, a.inner, a.so, a.si);
-  const Part<T> part(x, vocab, rank, cluster);
+  const Part<T, NT> part(x, vocab, rank, cluster);
   const RowStore<T> store(static_cast<T*>(a.grad) + r * a.vocab, part.row);
 
   // the teacher's slots, one a thread
+  const bool counted = a.row_mask == nullptr || a.row_mask[r];
   int id = -1;
   float l = -CUDART_INF_F;
-  if (tid < k && (a.row_mask == nullptr || a.row_mask[r])) {
+  if (tid < k && counted) {
     const int64_t id64 = a.teacher_ids[r * k + tid];
     id = id64 < 0 ? -1 : id64 >= vocab ? vocab : (int)id64;
-    if (id >= 0) l = a.teacher_logprobs[r * k + tid];
+    l = a.teacher_logprobs[r * k + tid];
+  }
+  if (kKeep && counted) {
+    for (int first = part.j0; first < part.j1; first += kVectors * NT) {
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) {
+        const int j = first + i * NT + tid;
+        if (j < part.j1 && part.row.whole(j)) copy16_async(s_kept + (j - part.j0), part.row.base + (int64_t)j * V::kVec);
+      }
+      if (first == part.j0) copies_commit();
+    }
+    copies_commit();
+    for (int e = 0; e < 2; ++e) {  // the ends of the row, where they are not whole
+      const int j = e == 0 ? 0 : part.row.count() - 1;
+      if (j >= part.j0 && j < part.j1 && !part.row.whole(j) && (j - part.j0) % NT == tid)
+        s_kept[j - part.j0] = part.row.load(j);
+    }
   }
   const int words = ((part.j1 - part.j0) * V::kVec + 31) / 32;
-  for (int i = tid; i < words; i += kRowThreads) listed[i] = 0;
+  for (int i = tid; i < words; i += NT) listed[i] = 0;
   if (tid < k) s_id[tid] = id;
+  if (tid == 0) s_flags = s_listed = 0;
+  if (id < 0) l = -CUDART_INF_F;
   const bool used = __syncthreads_or(id >= 0);
   if (cluster > 1) cluster_wait();
   if (!used) {  // the same for the whole cluster
     if (tid == 0 && rank == 0 && a.loss != nullptr) a.loss[r] = 0.0f;
     if (a.grad != nullptr)
-      for (int j = part.j0 + tid; j < part.j1; j += kRowThreads) store.zero(j);
+      for (int j = part.j0 + tid; j < part.j1; j += NT) store.zero(j);
+    if (kKeep) copies_wait<0>();
     return;
   }
   const bool mine = id >= 0 && id < vocab && part.holds(id);
-  bool again = false;  // an id that another slot has too
   if (mine) {
     const int at = id + part.row.lead - part.j0 * V::kVec;
-    again = (atomicOr(&listed[at >> 5], 1u << (at & 31)) >> (at & 31)) & 1u;
+    const uint32_t bit = 1u << (at & 31);
+    if (atomicOr(&listed[at >> 5], bit) & bit) atomicOr(&s_flags, 1);  // an id that another slot has too
   }
+  if (id >= vocab) atomicOr(&s_flags, 2);
   const float xv = to_f32(x[id >= 0 && id < vocab ? id : 0]);
-  const bool off = __syncthreads_or(id >= vocab);
-  // log p of each slot, and the rest: 1 - sum p in 64 bits, for it may be far below 1
-  float rest = 0.0f;
+  // sum p for a teacher with a tail, in 64 bits (the rest, 1 - sum p, may be far below 1); else the
+  // list's maximum and the sum relative to it
   if (a.tail) {
-    const double sum = block_reduce<kRowThreads>(id >= 0 ? exp((double)l) : 0.0, sd, AddOp());
-    rest = (float)fmax(0.0, 1.0 - sum);
-    if (sum != sum) rest = CUDART_NAN_F;
+    const double sum = warp_sum(id >= 0 ? exp((double)l) : 0.0);
+    if (lane == 0) s_sum[warp] = sum;
   } else {
-    const float top = block_reduce<kRowThreads>(l, sf, MaxOp());
-    const float sum = block_reduce<kRowThreads>(id >= 0 && top > -CUDART_INF_F ? expf(l - top) : 0.0f, sf, AddOp());
-    l = l - top - logf(sum);
+    const float top = warp_max(l);
+    const float sum = warp_sum(l > -CUDART_INF_F ? expf(l - top) : l == l ? 0.0f : l);
+    if (lane == 0) s_top[warp] = top, s_sum[warp] = sum;
   }
-  const float p = id >= 0 ? expf(l) : 0.0f;
-  if (tid < k) s_p[tid] = p;
-  float weight = block_reduce<kRowThreads>(p, sf, AddOp());
-  if (k >= vocab) {  // every id may be listed: nothing is left to be the rest
-    float ones = 0.0f;
-    for (int i = tid; i < words; i += kRowThreads) ones += __popc(listed[i]);
-    if (block_reduce<kRowThreads>(ones, sf, AddOp()) == (float)vocab) rest = 0.0f;
-  }
-  weight = off ? CUDART_NAN_F : weight + rest;
-  const bool repeated = __syncthreads_or(again);
+  __syncthreads();
 
   const float c2 = a.inv_temperature * kLog2e;
   const float2 cc = make_float2(c2, c2);
   float m = -CUDART_INF_F;
   float2 sum = make_float2(0.0f, 0.0f), sum_list = sum;  // the ids not listed; those listed
-  for (int first = part.j0; first < part.j1; first += kVectors * kRowThreads) {
+  for (int first = part.j0; first < part.j1; first += kVectors * NT) {
     uint4 v[kVectors];
-    part.load(first, v);
+    if (kKeep) {
+      if (first == part.j0) copies_wait<1>(); else copies_wait<0>();
+      part.load_from(s_kept, first, v);
+    } else {
+      part.load(first, v);
+    }
     typename V::Max mv = V::max_of(v[0]);
 #pragma unroll
     for (int i = 1; i < kVectors; ++i) mv = V::join(mv, V::max_of(v[i]));
@@ -112,10 +138,10 @@ __global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
     const float s = m == -CUDART_INF_F ? 0.0f : -m;
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
-      if (first + i * kRowThreads >= part.j1) break;
-      const int at = (first - part.j0 + i * kRowThreads + tid) * V::kVec;
+      if (first + i * NT >= part.j1) break;
+      const int at = (first - part.j0 + i * NT + tid) * V::kVec;
       uint32_t bits = 0;
-      if (first + i * kRowThreads + tid < part.j1)
+      if (first + i * NT + tid < part.j1)
         bits = (reinterpret_cast<const unsigned char*>(listed)[at >> 3] >> (at & 7)) & ((1u << V::kVec) - 1u);
       float2 e[V::kVec / 2];
       V::unpack(v[i], e);
@@ -135,20 +161,18 @@ __global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
       for (int h = 0; h < V::kVec / 2; ++h) sum = add2(sum, e[h]);
     }
   }
-  const float w_rest_sum = warp_sum(sum.x + sum.y), w_list_sum = warp_sum(sum_list.x + sum_list.y);
-  if (lane == 0) s_m[warp] = m, s_rest[warp] = w_rest_sum, s_list[warp] = w_list_sum;
+  if (kKeep) copies_wait<0>();
+  float s_r = warp_sum(sum.x + sum.y), s_l = warp_sum(sum_list.x + sum_list.y);
+  if (lane == 0) s_m[warp] = m, s_rest[warp] = s_r, s_list[warp] = s_l;
+  if (k >= vocab) {  // every id may be listed: nothing is left to be the rest
+    for (int i = tid; i < words; i += NT) atomicAdd(&s_listed, __popc(listed[i]));
+  }
   __syncthreads();
   // every warp joins the warps' sums, then the parts' sums, in the same order
-  auto join = [&](float& jm, float& jr, float& jl) {
-    const float top = warp_max(jm);
-    const float f = ex2_approx((jm - (top == -CUDART_INF_F ? 0.0f : top)) * c2);
-    jm = top;
-    jr = warp_sum(jr == 0.0f ? 0.0f : f * jr);
-    jl = warp_sum(jl == 0.0f ? 0.0f : f * jl);
-  };
-  float s_r = lane < kWarps ? s_rest[lane] : 0.0f, s_l = lane < kWarps ? s_list[lane] : 0.0f;
+  s_r = lane < kWarps ? s_rest[lane] : 0.0f;
+  s_l = lane < kWarps ? s_list[lane] : 0.0f;
   m = lane < kWarps ? s_m[lane] : -CUDART_INF_F;
-  join(m, s_r, s_l);
+  warp_join(c2, m, s_r, s_l);
   if (cluster > 1) {
     if (tid < 3 * cluster)
       st_cluster(cluster_address(&s_parts[rank][tid % 3], tid / 3), tid % 3 == 0 ? m : tid % 3 == 1 ? s_r : s_l);
@@ -157,49 +181,81 @@ __global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
     m = lane < cluster ? s_parts[lane][0] : -CUDART_INF_F;
     s_r = lane < cluster ? s_parts[lane][1] : 0.0f;
     s_l = lane < cluster ? s_parts[lane][2] : 0.0f;
-    join(m, s_r, s_l);
+    warp_join(c2, m, s_r, s_l);
   }
   if (m == -CUDART_INF_F) m = 0.0f;
   const float total = s_r + s_l, ln_total = log2f(total) * kLn2;
+  // the teacher: log p of the slot, sum p + rest, the rest
+  const bool off = s_flags & 2;
+  float weight = 1.0f, rest = 0.0f;
+  if (a.tail) {
+    double sum_p = 0.0;
+#pragma unroll
+    for (int w = 0; w < DWARF_TOP_K_MAX / 32; ++w) sum_p += s_sum[w];
+    rest = (float)fmax(0.0, 1.0 - sum_p);
+    if (s_listed == vocab) rest = 0.0f;
+    weight = (float)(sum_p + (double)rest);
+    if (sum_p != sum_p) rest = weight = CUDART_NAN_F;
+  } else {
+    float top = -CUDART_INF_F, sum_p = 0.0f;
+#pragma unroll
+    for (int w = 0; w < DWARF_TOP_K_MAX / 32; ++w) top = fmaxf(top, s_top[w]);
+#pragma unroll
+    for (int w = 0; w < DWARF_TOP_K_MAX / 32; ++w)
+      sum_p += s_sum[w] == 0.0 ? 0.0f : (float)s_sum[w] * expf(s_top[w] - top);
+    l = l - top - logf(sum_p);
+    if (!(sum_p > 0.0f)) weight = CUDART_NAN_F;  // no slot with a finite value
+  }
+  if (off) weight = CUDART_NAN_F;
+  const float p = id >= 0 ? expf(l) : 0.0f;
   if (a.loss != nullptr && rank == 0) {
     float term = p > 0.0f ? p * (l - (xv - m) * a.inv_temperature + ln_total) : p;
-    term = block_reduce<kRowThreads>(term, sf, AddOp());
-    if (tid == 0) {
-      if (!(rest <= 0.0f)) term += rest * (logf(rest) - log2f(s_r) * kLn2 + ln_total);
-      a.loss[r] = off ? CUDART_NAN_F : term * a.loss_scale;
-    }
+    term = warp_sum(term);
+    if (lane == 0) s_term[warp] = term;
   }
-  if (a.grad == nullptr) return;
-  const float sc = scale * a.inv_temperature;
-  const float k_list = sc * weight / total;
-  const float k_rest = rest > 0.0f && s_r > 0.0f ? sc * (weight / total - rest / s_r) : k_list;
-  const float2 shift = make_float2(-m, -m);
-  for (int first = part.j0; first < part.j1; first += kVectors * kRowThreads) {
-    uint4 v[kVectors];
-    part.load(first, v);
+  if (tid < k) s_p[tid] = p;
+  if (a.grad != nullptr) {
+    const float sc = scale * a.inv_temperature;
+    const float k_list = sc * weight / total;
+    const float k_rest = rest > 0.0f && s_r > 0.0f ? sc * (weight / total - rest / s_r) : k_list;
+    const float2 shift = make_float2(-m, -m);
+    for (int first = part.j0; first < part.j1; first += kVectors * NT) {
+      uint4 v[kVectors];
+      if (kKeep) part.load_from(s_kept, first, v); else part.load(first, v);
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      const int j = first + i * kRowThreads + tid;
-      if (j >= part.j1) break;
-      float2 e[V::kVec / 2];
-      V::unpack(v[i], e);
+      for (int i = 0; i < kVectors; ++i) {
+        const int j = first + i * NT + tid;
+        if (j >= part.j1) break;
+        float2 e[V::kVec / 2];
+        V::unpack(v[i], e);
 #pragma unroll
-      for (int h = 0; h < V::kVec / 2; ++h) {
-        const float2 d = mul2(add2(e[h], shift), cc);
-        e[h] = mul2(make_float2(ex2_approx(d.x), ex2_approx(d.y)), make_float2(k_rest, k_rest));
+        for (int h = 0; h < V::kVec / 2; ++h) {
+          const float2 d = mul2(add2(e[h], shift), cc);
+          e[h] = mul2(make_float2(ex2_approx(d.x), ex2_approx(d.y)), make_float2(k_rest, k_rest));
+        }
+        store.put(j, V::pack(e));
       }
-      store.put(j, V::pack(e));
     }
+    __syncthreads();  // the listed entries are written again, with their own terms
+    if (mine) {
+      float taken = p;
+      if (s_flags & 1) {
+        taken = 0.0f;
+        for (int j = 0; j < k; ++j)
+          if (s_id[j] == id) taken += s_p[j];
+      }
+      store.out[id] = from_f32<T>(ex2_approx((xv - m) * c2) * k_list - sc * taken);
+    }
+  } else {
+    __syncthreads();
   }
-  __syncthreads();  // the listed entries are written again, with their own terms
-  if (!mine) return;
-  float taken = p;
-  if (repeated) {
-    taken = 0.0f;
-    for (int j = 0; j < k; ++j)
-      if (s_id[j] == id) taken += s_p[j];
+  if (a.loss != nullptr && rank == 0 && tid == 0) {
+    float term = 0.0f;
+#pragma unroll
+    for (int w = 0; w < DWARF_TOP_K_MAX / 32; ++w) term += s_term[w];
+    if (!(rest <= 0.0f)) term += rest * (logf(rest) - log2f(s_r) * kLn2 + ln_total);
+    a.loss[r] = off ? CUDART_NAN_F : term * a.loss_scale;
   }
-  store.out[id] = from_f32<T>(ex2_approx((xv - m) * c2) * k_list - sc * taken);
 }
 
 __global__ void __launch_bounds__(1024) row_reduce_kernel(dwarf_row_reduce_args a) {
@@ -220,10 +276,27 @@ template <typename T>
 int launch_distill(const dwarf_topk_distill_args& a, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner;
   const int vectors = ceil_div((int)a.vocab, Vec16<T>::kVec);
+  const char* e = getenv("DWARF_X");
+  const int nt = e ? atoi(e) : 0;
+  const int keep = 4096;
+  if (a.grad != nullptr && vectors <= kMaxCluster * keep && nt != 1) {
+    const int cluster = cluster_for(rows, vectors, keep);
+    // a row that starts off a 16-byte boundary has one vector more
+    const int per = ceil_div(vectors + 1, cluster), bits_at = per * 16;
+    const int bytes = bits_at + (per * Vec16<T>::kVec + 31) / 32 * 4;
+    auto go = [&](auto kernel, int threads) {
+      if (bytes > 32 * 1024 &&
+          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+        return launch_status();
+      return launch_rows(kernel, rows, cluster, threads, bytes, stream, a, cluster, bits_at);
+    };
+    if (nt == 128) return go(topk_distill_kernel<T, 128, true>, 128);
+    if (nt == 512) return go(topk_distill_kernel<T, 512, true>, 512);
+    return go(topk_distill_kernel<T, 256, true>, 256);
+  }
   const int cluster = cluster_for(rows, vectors, 262144 / Vec16<T>::kVec);  // a bit for each place: at most 32 KB
-  // a row that starts off a 16-byte boundary has one vector more
   const int bytes = (ceil_div(vectors + 1, cluster) * Vec16<T>::kVec + 31) / 32 * 4;
-  return launch_rows(topk_distill_kernel<T>, rows, cluster, kRowThreads, bytes, stream, a, cluster);
+  return launch_rows(topk_distill_kernel<T, 128, false>, rows, cluster, 128, bytes, stream, a, cluster, 0);
 }
 
 }  // namespace

@@ -12,7 +12,7 @@ namespace {
 
 constexpr int kGroups = 2 * kRowThreads;
 constexpr int kCandidates = 512;    // entries that the search for the alternatives sorts
-constexpr int kHits = 512;          // vectors that it looks through
+constexpr int kHits = 512;          // cells that it looks through
 
 // What a softmax needs of a part of a row: the maximum, S and T relative to it.
 struct Sums {
@@ -31,85 +31,109 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
 }
 
+// How many of the n keys are above `key`.
+__device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int n) {
+  int above = 0;
+  const ulonglong2* q = reinterpret_cast<const ulonglong2*>(keys);
+#pragma unroll 4
+  for (int i = 0; i < n / 2; ++i) {
+    const ulonglong2 w = q[i];
+    above += (w.x > key) + (w.y > key);
+  }
+  if (n & 1) above += keys[n - 1] > key;
+  return above;
+}
+
 struct TopShared {
   uint32_t value[kGroups];           // order keys of the maxima, two of each thread
-  int hit[kHits];                    // vectors that reach the bound
-  uint64_t candidate[kCandidates];
+  int hit[kHits];                    // cells that reach the bound
+  alignas(16) uint64_t candidate[kCandidates];
   uint32_t bound;
   int n, hits;
   int scan[kRowThreads / 32];
 };
 
-// A bound that K entries of the part reach: the smallest of the group maxima that the
-// K-th largest 16-bit prefix among them takes in. With G >= 2 K groups and entries in random
-// places about G ln(G / (G - K)) entries reach it. One warp searches the prefix bit by bit
-// (a rank of each group by comparison with all others took five times the instructions).
-__device__ __forceinline__ uint32_t bound_of_groups(const uint32_t* value, int k) {
-  const int lane = threadIdx.x & 31;
-  uint32_t g[kGroups / 32];
+// The smallest of the group maxima that the K-th largest 16-bit prefix among them takes in;
+// one warp, kPer groups a lane. The search starts below the bits that all groups share.
+template <int kPer>
+__device__ __forceinline__ uint32_t bound_of(const uint32_t (&g)[kPer], int k) {
+  uint32_t high = g[0], low = g[0];
 #pragma unroll
-  for (int i = 0; i < kGroups / 32; ++i) g[i] = value[lane + 32 * i];
-  int groups = kGroups;
-#pragma unroll
-  for (int half = kGroups / 64; half >= 1; half /= 2) {
-    if (groups < 4 * k) break;
-    groups /= 2;
-#pragma unroll
-    for (int i = 0; i < half; ++i) g[i] = max(g[i], g[i + half]), g[i + half] = 0;
-  }
-  uint32_t prefix = 0;
-#pragma unroll
-  for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+  for (int i = 1; i < kPer; ++i) high = max(high, g[i]), low = min(low, g[i]);
+  high = __reduce_max_sync(0xffffffffu, high);
+  low = __reduce_min_sync(0xffffffffu, low);
+  const uint32_t free = high == low ? 0u : 0xffffffffu >> __clz(high ^ low);  // the bits that differ, and all below
+  uint32_t prefix = high & ~free;
+  for (uint32_t bit = free ^ (free >> 1); bit >= 0x10000u; bit >>= 1) {
     int c = 0;
 #pragma unroll
-    for (int i = 0; i < kGroups / 32; ++i) c += g[i] >= (prefix | bit);
+    for (int i = 0; i < kPer; ++i) c += g[i] >= (prefix | bit);
     if (__reduce_add_sync(0xffffffffu, c) >= k) prefix |= bit;
   }
   uint32_t least = 0xffffffffu;
 #pragma unroll
-  for (int i = 0; i < kGroups / 32; ++i)
-    if (g[i] >= prefix && g[i] > 0) least = min(least, g[i]);
+  for (int i = 0; i < kPer; ++i)
+    if (g[i] >= prefix) least = min(least, g[i]);
   return __reduce_min_sync(0xffffffffu, least);
 }
 
+// A bound that K entries of the part reach, from the maxima of G >= 2 K groups (K <= G suffices):
+// with entries in random places about G ln(G / (G - K)) reach it.
+__device__ __forceinline__ uint32_t bound_of_groups(const uint32_t* value, int k) {
+  const int lane = threadIdx.x & 31;
+  uint32_t g8[8], g4[4], g2[2], g1[1];
+  static_assert(kGroups == 256, "eight groups a lane");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) g8[i] = value[lane + 32 * i];
+  if (k > 64) return bound_of<8>(g8, k);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) g4[i] = max(g8[i], g8[i + 4]);
+  if (k > 32) return bound_of<4>(g4, k);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) g2[i] = max(g4[i], g4[i + 2]);
+  if (k > 16) return bound_of<2>(g2, k);
+  g1[0] = max(g2[0], g2[1]);
+  return bound_of<1>(g1, k);
+}
+
 // The K best entries of the part (order: value, then lowest id) among the first n
-// candidates, n >= min(K, entries of the part). `largest` holds 16 bits for each vector that are no
-// lower than its largest entry. The vectors that reach the bound are read again (from
-// L2) and their entries that reach it become candidates. Where these are more than the
-// buffers hold (ties, or many large values in one group), or a NaN is in the row, the
-// K-th value is found bit by bit over the whole part and its ties are taken in order.
+// candidates, n >= min(K, entries of the part). `cells` holds 16 bits, no lower than the
+// largest entry, for each cell: the even or the odd ones of a thread's vectors of a tile. The cells
+// that reach the bound are read again (from L2) and their entries that reach it become
+// candidates. Where these are more than the buffers hold (ties, or many large values in
+// one group), or a NaN is in the row, the K-th value is found bit by bit over the whole
+// part and its ties are taken in order.
 template <typename T>
-__device__ __forceinline__ int best_entries(const Part<T>& part, const typename Vec16<T>::Narrow* largest, int k,
+__device__ __forceinline__ int best_entries(const Part<T>& part, const typename Vec16<T>::Narrow* cells, int k,
                                             bool nan, TopShared& sh) {
   using N16 = Vec16<typename Vec16<T>::Narrow>;
   const int tid = threadIdx.x;
   uint32_t limit = sh.bound;
   if (!nan) {
     const float bound = key_value(limit);
-    const int n = part.j1 - part.j0;
+    const int n = ceil_div(part.j1 - part.j0, kVectors * kRowThreads) * kGroups;
     for (int c = 8 * tid; c < n; c += 8 * kRowThreads) {
-      const uint4 w = *reinterpret_cast<const uint4*>(largest + c);
-      if (!N16::reaches(N16::max_of(w), bound)) continue;
-      const typename Vec16<T>::Narrow* e = reinterpret_cast<const typename Vec16<T>::Narrow*>(&w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (c + i < n && to_f32(e[i]) >= bound) {
-          const int at = atomicAdd(&sh.hits, 1);
-          if (at < kHits) sh.hit[at] = part.j0 + c + i;
-        }
+      const uint4 w = *reinterpret_cast<const uint4*>(cells + c);
+      for (uint32_t m = N16::reach(w, bound); m != 0; m &= m - 1) {
+        const int at = atomicAdd(&sh.hits, 1);
+        if (at < kHits) sh.hit[at] = c + N16::element(__ffs(m) - 1);
       }
     }
     __syncthreads();
     const int hits = sh.hits;
     if (hits <= kHits) {
-      for (int h = tid; h < hits; h += kRowThreads) {
-        const int j = sh.hit[h];
-        part.elements(part.row.load(j), j, [&](float x, int id) {
-          if (x >= bound) {
-            const int at = atomicAdd(&sh.n, 1);
-            if (at < kCandidates) sh.candidate[at] = entry_key(x, (uint32_t)id);
-          }
-        });
+      constexpr int kCell = kVectors / 2;
+      for (int h = tid; h < hits * kCell; h += kRowThreads) {
+        const int c = sh.hit[h / kCell];  // [tile][thread][even, odd]
+        const int j = part.j0 + (c / kGroups * kVectors + 2 * (h % kCell) + (c & 1)) * kRowThreads + (c % kGroups) / 2;
+        if (j >= part.j1) continue;
+        const uint4 w = part.row.load(j);
+        for (uint32_t m = Vec16<T>::reach(w, bound); m != 0; m &= m - 1) {
+          const int e = Vec16<T>::element(__ffs(m) - 1), u = j * Part<T>::kVec + e;
+          if (u < part.row.lead || u >= part.row.end) continue;
+          const int at = atomicAdd(&sh.n, 1);
+          if (at < kCandidates) sh.candidate[at] = entry_key(Vec16<T>::value(w, e), (uint32_t)(u - part.row.lead));
+        }
       }
       __syncthreads();
       if (sh.n <= kCandidates) return sh.n;
@@ -184,12 +208,12 @@ __device__ __forceinline__ int best_entries(const Part<T>& part, const typename 
 // another's sums and search; 512 threads that hold a whole row reached 4.0 of these
 // 6.4 TB/s (16384 rows of 32768 bf16, no alternatives).
 template <typename T, bool kTop>
-__global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 9)
     token_logprobs_kernel(const dwarf_token_logprobs_args a, int cluster, int lists_at) {
   using V = Vec16<T>;
   constexpr int kWarps = kRowThreads / 32;
   extern __shared__ __align__(16) unsigned char s_dynamic[];
-  typename V::Narrow* s_largest = reinterpret_cast<typename V::Narrow*>(s_dynamic);
+  typename V::Narrow* s_cells = reinterpret_cast<typename V::Narrow*>(s_dynamic);
   uint64_t* s_lists = reinterpret_cast<uint64_t*>(s_dynamic + lists_at);  // [cluster][k], in rank 0
   __shared__ Sums s_warp[kWarps];
   __shared__ float s_parts[kMaxCluster][3];
@@ -215,13 +239,14 @@ __global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
     for (int i = 0; i < kVectors; ++i) {
       const typename V::Max of = V::max_of(v[i]);
       mv[i & 1] = i < 2 ? of : V::join(mv[i & 1], of);
-      const int j = first - part.j0 + i * kRowThreads + tid;
-      if (kTop && j < part.j1 - part.j0) s_largest[j] = V::narrow(of);
     }
     const float mx = V::largest(V::join(mv[0], mv[1]));
     if (kTop) {
       top0 = fmaxf(top0, V::largest(mv[0]));
       top1 = fmaxf(top1, V::largest(mv[1]));
+      typename V::Narrow* cell = s_cells + (first - part.j0) / kVectors * 2 + 2 * tid;
+      cell[0] = V::narrow(mv[0]);
+      cell[1] = V::narrow(mv[1]);
     }
     const float m = fmaxf(sum.m, warp_max(mx));
     if (sum.m > -CUDART_INF_F) {  // a later tile: move the sums to the new maximum
@@ -292,7 +317,7 @@ __global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
     bool nan = false;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) nan |= s_warp[w].s != s_warp[w].s;
-    n = best_entries(part, s_largest, k, nan, top);
+    n = best_entries(part, s_cells, k, nan, top);
   }
   if (cluster > 1) {
     if (kTop) {
@@ -301,8 +326,7 @@ __global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
         int at = c;
         if (c < n) {
           key = top.candidate[c];
-          at = 0;
-          for (int i = 0; i < n; ++i) at += top.candidate[i] > key;
+          at = rank_of(key, top.candidate, n);
         }
         if (at < k) st_cluster(cluster_address(&s_lists[rank * k + at], 0), key);
       }
@@ -348,8 +372,7 @@ __global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
   if (cluster == 1) {
     for (int c = tid; c < n; c += kRowThreads) {
       const uint64_t key = top.candidate[c];
-      int at = 0;
-      for (int i = 0; i < n; ++i) at += top.candidate[i] > key;
+      const int at = rank_of(key, top.candidate, n);
       if (at < k) put(key, at);
     }
   } else {
@@ -375,11 +398,11 @@ template <typename T>
 int launch_forward(const dwarf_token_logprobs_args& a, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner;
   const int vectors = ceil_div((int)a.vocab, Vec16<T>::kVec);
-  const int cluster = cluster_for(rows, vectors, 32768);  // vector maxima: at most 64 KB
+  const int cluster = cluster_for(rows, vectors, 65536);  // cells: at most 32 KB
   if (a.top_k == 0)
     return launch_rows(token_logprobs_kernel<T, false>, rows, cluster, kRowThreads, 0, stream, a, cluster, 0);
   // a row that starts off a 16-byte boundary has one vector more
-  const int lists_at = (ceil_div(vectors + 1, cluster) * 2 + 15) / 16 * 16;
+  const int lists_at = ceil_div(ceil_div(vectors + 1, cluster), kVectors * kRowThreads) * kGroups * 2;
   const int bytes = lists_at + (cluster > 1 ? cluster * a.top_k * 8 : 0);
   const auto kernel = token_logprobs_kernel<T, true>;
   if (bytes > 32 * 1024 &&

@@ -69,28 +69,10 @@ struct MaxOp {
   __device__ __forceinline__ uint64_t operator()(uint64_t a, uint64_t b) const { return a > b ? a : b; }
 };
 
-// Packed pairs of fp32 (one issue slot for two elements).
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("{.reg .b64 pa, pb, pr;\nmov.b64 pa, {%2, %3};\nmov.b64 pb, {%4, %5};\n"
-      "add.rn.f32x2 pr, pa, pb;\nmov.b64 {%0, %1}, pr;\n}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("{.reg .b64 pa, pb, pr;\nmov.b64 pa, {%2, %3};\nmov.b64 pb, {%4, %5};\n"
-      "mul.rn.f32x2 pr, pa, pb;\nmov.b64 {%0, %1}, pr;\n}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{.reg .b64 pa, pb, pc;\nmov.b64 pa, {%2, %3};\nmov.b64 pb, {%4, %5};\nmov.b64 pc, {%6, %7};\n"
-      "fma.rn.f32x2 pc, pa, pb, pc;\nmov.b64 {%0, %1}, pc;\n}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
+// Pairs of fp32: one issue slot for two elements.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 
 // 16 bytes of a row: kVec elements.
 template <typename T>
@@ -117,7 +99,15 @@ struct Vec16<float> {
   __device__ __forceinline__ static float largest(Max a) { return a; }
   using Narrow = __nv_bfloat16;  // 16 bits that are no lower than the largest
   __device__ __forceinline__ static Narrow narrow(Max a) { return __float2bfloat16_ru(a); }
-  __device__ __forceinline__ static bool reaches(Max a, float bound) { return a >= bound; }
+  // The elements of at least `bound` (the nearest lower value of the type) as bits; the element of a bit; its value.
+  __device__ __forceinline__ static uint32_t reach(const uint4& v, float bound) {
+    return (uint32_t)(__uint_as_float(v.x) >= bound) | (uint32_t)(__uint_as_float(v.y) >= bound) << 1 |
+           (uint32_t)(__uint_as_float(v.z) >= bound) << 2 | (uint32_t)(__uint_as_float(v.w) >= bound) << 3;
+  }
+  __device__ __forceinline__ static int element(int bit) { return bit; }
+  __device__ __forceinline__ static float value(const uint4& v, int e) {
+    return __uint_as_float(e & 2 ? (e & 1 ? v.w : v.z) : (e & 1 ? v.y : v.x));
+  }
   // Elements no lower than `low`.
   using Low = float;
   __device__ __forceinline__ static Low low_of(float v) { return v; }
@@ -162,7 +152,17 @@ struct Vec16<__nv_bfloat16> {
     const float2 f = __bfloat1622float2(a);
     return fmaxf(f.x, f.y);
   }
-  __device__ __forceinline__ static bool reaches(Max a, float bound) { return largest(a) >= bound; }
+  __device__ __forceinline__ static uint32_t reach(const uint4& v, float bound) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const __nv_bfloat162 b = __bfloat162bfloat162(__float2bfloat16_rd(bound));
+    return (__hge2_mask(h[0], b) & 0x00010001u) | (__hge2_mask(h[1], b) & 0x00020002u) |
+           (__hge2_mask(h[2], b) & 0x00040004u) | (__hge2_mask(h[3], b) & 0x00080008u);
+  }
+  __device__ __forceinline__ static int element(int bit) { return 2 * (bit & 15) + (bit >> 4); }
+  __device__ __forceinline__ static float value(const uint4& v, int e) {
+    const uint32_t w = e & 4 ? (e & 2 ? v.w : v.z) : (e & 2 ? v.y : v.x);
+    return to_f32(__ushort_as_bfloat16((unsigned short)(e & 1 ? w >> 16 : w & 0xffffu)));
+  }
   using Low = __nv_bfloat162;
   __device__ __forceinline__ static Low low_of(float v) { return __float2bfloat162_rn(v); }
   __device__ __forceinline__ static float low_value(Low low) { return __low2float(low); }
@@ -206,7 +206,17 @@ struct Vec16<__half> {
     const float2 f = __half22float2(a);
     return fmaxf(f.x, f.y);
   }
-  __device__ __forceinline__ static bool reaches(Max a, float bound) { return largest(a) >= bound; }
+  __device__ __forceinline__ static uint32_t reach(const uint4& v, float bound) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    const __half2 b = __half2half2(__float2half_rd(bound));
+    return (__hge2_mask(h[0], b) & 0x00010001u) | (__hge2_mask(h[1], b) & 0x00020002u) |
+           (__hge2_mask(h[2], b) & 0x00040004u) | (__hge2_mask(h[3], b) & 0x00080008u);
+  }
+  __device__ __forceinline__ static int element(int bit) { return 2 * (bit & 15) + (bit >> 4); }
+  __device__ __forceinline__ static float value(const uint4& v, int e) {
+    const uint32_t w = e & 4 ? (e & 2 ? v.w : v.z) : (e & 2 ? v.y : v.x);
+    return to_f32(__ushort_as_half((unsigned short)(e & 1 ? w >> 16 : w & 0xffffu)));
+  }
   using Low = __half2;
   __device__ __forceinline__ static Low low_of(float v) { return __float2half2_rn(v); }
   __device__ __forceinline__ static float low_value(Low low) { return __low2float(low); }
@@ -225,6 +235,18 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
+}
+
+// 16 bytes into shared memory without passing through registers.
+__device__ __forceinline__ void copy16_async(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits until at most kLeft of the thread's committed groups are in flight.
+template <int kLeft>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
 
 __device__ __forceinline__ void st_stream(void* p, const uint4& v) {
@@ -274,7 +296,8 @@ __device__ __forceinline__ float warp_max(float v) {
   return __int_as_float(k);
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
+template <typename V>
+__device__ __forceinline__ V warp_sum(V v) {
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
@@ -322,7 +345,7 @@ int launch_rows(void (*kernel)(Params...), int64_t rows, int cluster, int thread
 }
 
 // A CTA's part of a row, a tile of kVectors vectors for each thread at a time.
-template <typename T>
+template <typename T, int kThreads = kRowThreads>
 struct Part {
   static constexpr int kVec = Vec16<T>::kVec;
   RowVectors<T> row;
@@ -338,15 +361,24 @@ struct Part {
     const int j = first + threadIdx.x;
     const int lo = row.lead > 0 ? 1 : 0, hi = row.end / kVec;  // the whole vectors
     const uint4* p = reinterpret_cast<const uint4*>(row.base) + j;
-    if (first >= lo && first + kVectors * kRowThreads <= min(j1, hi)) {
+    if (first >= lo && first + kVectors * kThreads <= min(j1, hi)) {
 #pragma unroll
-      for (int i = 0; i < kVectors; ++i) v[i] = ld_stream(p + i * kRowThreads);
+      for (int i = 0; i < kVectors; ++i) v[i] = ld_stream(p + i * kThreads);
       return;
     }
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
       v[i] = make_uint4(Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf);
-      if (j + i * kRowThreads < j1) v[i] = row.load(j + i * kRowThreads);
+      if (j + i * kThreads < j1) v[i] = row.load(j + i * kThreads);
+    }
+  }
+  // The same from a copy of the part.
+  __device__ __forceinline__ void load_from(const uint4* kept, int first, uint4 (&v)[kVectors]) const {
+    const int j = first - j0 + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+      v[i] = make_uint4(Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf);
+      if (j + i * kThreads < j1 - j0) v[i] = kept[j + i * kThreads];
     }
   }
   __device__ __forceinline__ bool holds(int id) const {
@@ -367,7 +399,7 @@ struct Part {
   // f(vector, j, whether j is in the part), one step of the whole block after the other, in rising j.
   template <typename F>
   __device__ __forceinline__ void walk(F f) const {
-    for (int first = j0; first < j1; first += kRowThreads) {
+    for (int first = j0; first < j1; first += kThreads) {
       const int j = first + threadIdx.x;
       uint4 w = make_uint4(0, 0, 0, 0);
       if (j < j1) w = row.load(j);
