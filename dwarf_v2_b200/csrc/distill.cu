@@ -21,76 +21,57 @@ __device__ __forceinline__ void warp_join(float c2, float& m, float& a, float& b
   b = warp_sum(b == 0.0f ? 0.0f : f * b);
 }
 
-// kKeep: the part's vectors stay in shared memory between the sums and the gradient; every
-// thread reads back only what it copied there itself. Otherwise they are read again.
-template <typename T, int NT, bool kKeep>
-__global__ void __launch_bounds__(NT, (kKeep ? 768 : 1024) / NT)
-    topk_distill_kernel(const dwarf_topk_distill_args a, int cluster, int bits_at) {
+// One CTA, or a cluster of them, for a row. With the gradient the row is read twice, the
+// second time from L2: one bulk prefetch at the start fetches the row while the teacher's list is
+// read, under a policy that keeps it there, and the threads of a CTA are chosen so that the
+// rows in flight are about 40 MB. 16384 rows of 32768 bf16, 64 entries: 388 us (128 threads
+// without either: 534, with 475 MB read for 268; the row held in shared memory: 483; 512
+// threads: 540). The loss alone: 128 threads, no prefetch, 196 us (256 threads: 249).
+template <typename T, int NT, bool kGrad>
+__global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_kernel(const dwarf_topk_distill_args a, int cluster) {
   using V = Vec16<T>;
-  constexpr int kWarps = NT / 32;
+  constexpr int kWarps = NT / 32, kTile = kVectors * NT, kListWarps = DWARF_TOP_K_MAX / 32;
   static_assert(NT >= DWARF_TOP_K_MAX, "one thread for each slot of the teacher's list");
-  extern __shared__ __align__(16) unsigned char s_dynamic[];
-  uint4* s_kept = reinterpret_cast<uint4*>(s_dynamic);
-  uint32_t* listed = reinterpret_cast<uint32_t*>(s_dynamic + bits_at);  // a bit for each place of the part
-  __shared__ float s_m[kWarps], s_rest[kWarps], s_list[kWarps], s_term[kWarps];
-  __shared__ float s_top[kWarps];
-  __shared__ double s_sum[kWarps];
+  extern __shared__ __align__(16) uint32_t listed[];  // a bit for each place of the part
+  __shared__ float s_m[kWarps], s_rest[kWarps], s_list[kWarps];
+  __shared__ float s_top[kListWarps], s_term[kListWarps];
+  __shared__ double s_sum[kListWarps];
   __shared__ float s_parts[kMaxCluster][3];
   __shared__ int s_id[DWARF_TOP_K_MAX];
   __shared__ float s_p[DWARF_TOP_K_MAX];
   __shared__ int s_flags, s_listed;
+  if (a.skip_if_one && *a.grad_rows == 1.0f) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int vocab = (int)a.vocab, k = a.k;
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
   const int64_t r = blockIdx.x / (unsigned)cluster;
-  float scale = a.scale * (a.grad_scale != nullptr ? *a.grad_scale : 1.0f);
-  if (a.grad_rows != nullptr) {
-    const float g = a.grad_rows[a.grad_rows_stride ? r : 0];
-    if (a.skip_if_one && g == 1.0f) return;
-    scale *= g;
-  }
   if (cluster > 1) cluster_arrive();  // its CTAs have started, before one writes to another
   const T* x = static_cast<const T*>(a.logits) + row_offset(r, a.inner, a.so, a.si);
   const Part<T, NT> part(x, vocab, rank, cluster);
-  const RowStore<T> store(static_cast<T*>(a.grad) + r * a.vocab, part.row);
+  const uint64_t keep = kGrad ? policy_keep() : 0;
 
   // the teacher's slots, one a thread
-  const bool counted = a.row_mask == nullptr || a.row_mask[r];
-  int id = -1;
+  const bool counted = a.row_mask == nullptr || a.row_mask[r] != 0;
+  if (kGrad && tid == 0 && counted) part.prefetch(keep);
+  int id = -1;  // not used; vocab: past the vocabulary
   float l = -CUDART_INF_F;
   if (tid < k && counted) {
     const int64_t id64 = a.teacher_ids[r * k + tid];
-    id = id64 < 0 ? -1 : id64 >= vocab ? vocab : (int)id64;
     l = a.teacher_logprobs[r * k + tid];
+    id = id64 < 0 ? -1 : id64 >= vocab ? vocab : (int)id64;
+    if (id < 0) l = -CUDART_INF_F;
   }
-  if (kKeep && counted) {
-    for (int first = part.j0; first < part.j1; first += kVectors * NT) {
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i) {
-        const int j = first + i * NT + tid;
-        if (j < part.j1 && part.row.whole(j)) copy16_async(s_kept + (j - part.j0), part.row.base + (int64_t)j * V::kVec);
-      }
-      if (first == part.j0) copies_commit();
-    }
-    copies_commit();
-    for (int e = 0; e < 2; ++e) {  // the ends of the row, where they are not whole
-      const int j = e == 0 ? 0 : part.row.count() - 1;
-      if (j >= part.j0 && j < part.j1 && !part.row.whole(j) && (j - part.j0) % NT == tid)
-        s_kept[j - part.j0] = part.row.load(j);
-    }
-  }
-  const int words = ((part.j1 - part.j0) * V::kVec + 31) / 32;
+  const int words = (part.size() * V::kVec + 31) / 32;
   for (int i = tid; i < words; i += NT) listed[i] = 0;
   if (tid < k) s_id[tid] = id;
   if (tid == 0) s_flags = s_listed = 0;
-  if (id < 0) l = -CUDART_INF_F;
+  const RowStore<T> store(static_cast<T*>(a.grad) + r * a.vocab, part.row);
   const bool used = __syncthreads_or(id >= 0);
   if (cluster > 1) cluster_wait();
   if (!used) {  // the same for the whole cluster
     if (tid == 0 && rank == 0 && a.loss != nullptr) a.loss[r] = 0.0f;
-    if (a.grad != nullptr)
-      for (int j = part.j0 + tid; j < part.j1; j += NT) store.zero(j);
-    if (kKeep) copies_wait<0>();
+    if (kGrad)
+      for (int at = 0; at < part.size(); at += kTile) store.zero(part, at);
     return;
   }
   const bool mine = id >= 0 && id < vocab && part.holds(id);
@@ -103,13 +84,15 @@ __global__ void __launch_bounds__(NT, (kKeep ? 768 : 1024) / NT)
   const float xv = to_f32(x[id >= 0 && id < vocab ? id : 0]);
   // sum p for a teacher with a tail, in 64 bits (the rest, 1 - sum p, may be far below 1); else the
   // list's maximum and the sum relative to it
-  if (a.tail) {
-    const double sum = warp_sum(id >= 0 ? exp((double)l) : 0.0);
-    if (lane == 0) s_sum[warp] = sum;
-  } else {
-    const float top = warp_max(l);
-    const float sum = warp_sum(l > -CUDART_INF_F ? expf(l - top) : l == l ? 0.0f : l);
-    if (lane == 0) s_top[warp] = top, s_sum[warp] = sum;
+  if (warp < kListWarps) {
+    if (a.tail) {
+      const double sum = warp_sum(id >= 0 ? exp((double)l) : 0.0);
+      if (lane == 0) s_sum[warp] = sum;
+    } else {
+      const float top = warp_max(l);
+      const float sum = warp_sum(l > -CUDART_INF_F ? expf(l - top) : l == l ? 0.0f : l);
+      if (lane == 0) s_top[warp] = top, s_sum[warp] = sum;
+    }
   }
   __syncthreads();
 
@@ -117,14 +100,9 @@ __global__ void __launch_bounds__(NT, (kKeep ? 768 : 1024) / NT)
   const float2 cc = make_float2(c2, c2);
   float m = -CUDART_INF_F;
   float2 sum = make_float2(0.0f, 0.0f), sum_list = sum;  // the ids not listed; those listed
-  for (int first = part.j0; first < part.j1; first += kVectors * NT) {
+  for (int at = 0; at < part.size(); at += kTile) {
     uint4 v[kVectors];
-    if (kKeep) {
-      if (first == part.j0) copies_wait<1>(); else copies_wait<0>();
-      part.load_from(s_kept, first, v);
-    } else {
-      part.load(first, v);
-    }
+    if (kGrad) part.load(at, v, keep); else part.load(at, v);
     typename V::Max mv = V::max_of(v[0]);
 #pragma unroll
     for (int i = 1; i < kVectors; ++i) mv = V::join(mv, V::max_of(v[i]));
@@ -136,32 +114,38 @@ __global__ void __launch_bounds__(NT, (kKeep ? 768 : 1024) / NT)
     }
     m = m_new;
     const float s = m == -CUDART_INF_F ? 0.0f : -m;
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      if (first + i * NT >= part.j1) break;
-      const int at = (first - part.j0 + i * NT + tid) * V::kVec;
-      uint32_t bits = 0;
-      if (first + i * NT + tid < part.j1)
-        bits = (reinterpret_cast<const unsigned char*>(listed)[at >> 3] >> (at & 7)) & ((1u << V::kVec) - 1u);
+    // the bits of a thread's vectors of a tile lie NT kVec / 8 bytes apart
+    const unsigned char* bits = reinterpret_cast<const unsigned char*>(listed) + (at + tid) * V::kVec / 8;
+    const int bits_shift = V::kVec == 4 ? 4 * (tid & 1) : 0;
+    auto add = [&](const uint4& w, uint32_t mask) {
       float2 e[V::kVec / 2];
-      V::unpack(v[i], e);
+      V::unpack(w, e);
 #pragma unroll
       for (int h = 0; h < V::kVec / 2; ++h) {
         const float2 d = mul2(add2(e[h], make_float2(s, s)), cc);
         e[h] = make_float2(ex2_approx(d.x), ex2_approx(d.y));
       }
-      if (bits != 0) {
+      if (mask != 0) {
 #pragma unroll
         for (int h = 0; h < V::kVec / 2; ++h) {
-          if (bits & (1u << (2 * h))) sum_list.x += e[h].x, e[h].x = 0.0f;
-          if (bits & (2u << (2 * h))) sum_list.y += e[h].y, e[h].y = 0.0f;
+          if (mask & (1u << (2 * h))) sum_list.x += e[h].x, e[h].x = 0.0f;
+          if (mask & (2u << (2 * h))) sum_list.y += e[h].y, e[h].y = 0.0f;
         }
       }
 #pragma unroll
       for (int h = 0; h < V::kVec / 2; ++h) sum = add2(sum, e[h]);
+    };
+    if (at + kTile <= part.size()) {
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i)
+        add(v[i], (bits[i * NT * V::kVec / 8] >> bits_shift) & ((1u << V::kVec) - 1u));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i)
+        if (at + i * NT + tid < part.size())
+          add(v[i], (bits[i * NT * V::kVec / 8] >> bits_shift) & ((1u << V::kVec) - 1u));
     }
   }
-  if (kKeep) copies_wait<0>();
   float s_r = warp_sum(sum.x + sum.y), s_l = warp_sum(sum_list.x + sum_list.y);
   if (lane == 0) s_m[warp] = m, s_rest[warp] = s_r, s_list[warp] = s_l;
   if (k >= vocab) {  // every id may be listed: nothing is left to be the rest
@@ -184,14 +168,14 @@ __global__ void __launch_bounds__(NT, (kKeep ? 768 : 1024) / NT)
     warp_join(c2, m, s_r, s_l);
   }
   if (m == -CUDART_INF_F) m = 0.0f;
-  const float total = s_r + s_l, ln_total = log2f(total) * kLn2;
+  const float total = s_r + s_l;
   // the teacher: log p of the slot, sum p + rest, the rest
   const bool off = s_flags & 2;
   float weight = 1.0f, rest = 0.0f;
   if (a.tail) {
     double sum_p = 0.0;
 #pragma unroll
-    for (int w = 0; w < DWARF_TOP_K_MAX / 32; ++w) sum_p += s_sum[w];
+    for (int w = 0; w < kListWarps; ++w) sum_p += s_sum[w];
     rest = (float)fmax(0.0, 1.0 - sum_p);
     if (s_listed == vocab) rest = 0.0f;
     weight = (float)(sum_p + (double)rest);
@@ -199,61 +183,59 @@ __global__ void __launch_bounds__(NT, (kKeep ? 768 : 1024) / NT)
   } else {
     float top = -CUDART_INF_F, sum_p = 0.0f;
 #pragma unroll
-    for (int w = 0; w < DWARF_TOP_K_MAX / 32; ++w) top = fmaxf(top, s_top[w]);
+    for (int w = 0; w < kListWarps; ++w) top = fmaxf(top, s_top[w]);
 #pragma unroll
-    for (int w = 0; w < DWARF_TOP_K_MAX / 32; ++w)
+    for (int w = 0; w < kListWarps; ++w)
       sum_p += s_sum[w] == 0.0 ? 0.0f : (float)s_sum[w] * expf(s_top[w] - top);
     l = l - top - logf(sum_p);
     if (!(sum_p > 0.0f)) weight = CUDART_NAN_F;  // no slot with a finite value
   }
   if (off) weight = CUDART_NAN_F;
   const float p = id >= 0 ? expf(l) : 0.0f;
-  if (a.loss != nullptr && rank == 0) {
-    float term = p > 0.0f ? p * (l - (xv - m) * a.inv_temperature + ln_total) : p;
-    term = warp_sum(term);
+  if (a.loss != nullptr && warp < kListWarps) {
+    const float term = warp_sum(p > 0.0f ? p * (l - (xv - m) * a.inv_temperature + log2f(total) * kLn2) : p);
     if (lane == 0) s_term[warp] = term;
   }
   if (tid < k) s_p[tid] = p;
-  if (a.grad != nullptr) {
-    const float sc = scale * a.inv_temperature;
-    const float k_list = sc * weight / total;
+  float sc = 0.0f, k_list = 0.0f;
+  if (kGrad) {
+    sc = a.scale * a.inv_temperature;
+    if (a.grad_scale != nullptr) sc *= *a.grad_scale;
+    if (a.grad_rows != nullptr) sc *= a.grad_rows[a.grad_rows_stride ? r : 0];
+    k_list = sc * weight / total;
     const float k_rest = rest > 0.0f && s_r > 0.0f ? sc * (weight / total - rest / s_r) : k_list;
     const float2 shift = make_float2(-m, -m);
-    for (int first = part.j0; first < part.j1; first += kVectors * NT) {
+    const uint64_t leave = policy_leave();
+    for (int at = 0; at < part.size(); at += kTile) {
       uint4 v[kVectors];
-      if (kKeep) part.load_from(s_kept, first, v); else part.load(first, v);
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i) {
-        const int j = first + i * NT + tid;
-        if (j >= part.j1) break;
+      part.load(at, v, leave);
+      store.tile(part, at, v, [&](const uint4& w) {
         float2 e[V::kVec / 2];
-        V::unpack(v[i], e);
+        V::unpack(w, e);
 #pragma unroll
         for (int h = 0; h < V::kVec / 2; ++h) {
           const float2 d = mul2(add2(e[h], shift), cc);
           e[h] = mul2(make_float2(ex2_approx(d.x), ex2_approx(d.y)), make_float2(k_rest, k_rest));
         }
-        store.put(j, V::pack(e));
-      }
+        return V::pack(e);
+      });
     }
-    __syncthreads();  // the listed entries are written again, with their own terms
-    if (mine) {
-      float taken = p;
-      if (s_flags & 1) {
-        taken = 0.0f;
-        for (int j = 0; j < k; ++j)
-          if (s_id[j] == id) taken += s_p[j];
-      }
-      store.out[id] = from_f32<T>(ex2_approx((xv - m) * c2) * k_list - sc * taken);
+  }
+  __syncthreads();  // the listed entries are written again, with their own terms
+  if (kGrad && mine) {
+    float taken = p;
+    if (s_flags & 1) {
+      taken = 0.0f;
+      for (int j = 0; j < k; ++j)
+        if (s_id[j] == id) taken += s_p[j];
     }
-  } else {
-    __syncthreads();
+    store.out[id] = from_f32<T>(ex2_approx((xv - m) * c2) * k_list - sc * taken);
   }
   if (a.loss != nullptr && rank == 0 && tid == 0) {
     float term = 0.0f;
 #pragma unroll
-    for (int w = 0; w < DWARF_TOP_K_MAX / 32; ++w) term += s_term[w];
-    if (!(rest <= 0.0f)) term += rest * (logf(rest) - log2f(s_r) * kLn2 + ln_total);
+    for (int w = 0; w < kListWarps; ++w) term += s_term[w];
+    if (!(rest <= 0.0f)) term += rest * (logf(rest) - (log2f(s_r) - log2f(total)) * kLn2);
     a.loss[r] = off ? CUDART_NAN_F : term * a.loss_scale;
   }
 }
@@ -276,27 +258,17 @@ template <typename T>
 int launch_distill(const dwarf_topk_distill_args& a, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner;
   const int vectors = ceil_div((int)a.vocab, Vec16<T>::kVec);
-  const char* e = getenv("DWARF_X");
-  const int nt = e ? atoi(e) : 0;
-  const int keep = 4096;
-  if (a.grad != nullptr && vectors <= kMaxCluster * keep && nt != 1) {
-    const int cluster = cluster_for(rows, vectors, keep);
-    // a row that starts off a 16-byte boundary has one vector more
-    const int per = ceil_div(vectors + 1, cluster), bits_at = per * 16;
-    const int bytes = bits_at + (per * Vec16<T>::kVec + 31) / 32 * 4;
-    auto go = [&](auto kernel, int threads) {
-      if (bytes > 32 * 1024 &&
-          cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-        return launch_status();
-      return launch_rows(kernel, rows, cluster, threads, bytes, stream, a, cluster, bits_at);
-    };
-    if (nt == 128) return go(topk_distill_kernel<T, 128, true>, 128);
-    if (nt == 512) return go(topk_distill_kernel<T, 512, true>, 512);
-    return go(topk_distill_kernel<T, 256, true>, 256);
-  }
   const int cluster = cluster_for(rows, vectors, 262144 / Vec16<T>::kVec);  // a bit for each place: at most 32 KB
-  const int bytes = (ceil_div(vectors + 1, cluster) * Vec16<T>::kVec + 31) / 32 * 4;
-  return launch_rows(topk_distill_kernel<T, 128, false>, rows, cluster, 128, bytes, stream, a, cluster, 0);
+  // a row that starts off a 16-byte boundary has one vector more
+  const int part = ceil_div(vectors + 1, cluster);
+  const int bytes = (part * Vec16<T>::kVec + 31) / 32 * 4;
+  if (a.grad == nullptr)
+    return launch_rows(topk_distill_kernel<T, 128, false>, rows, cluster, 128, bytes, stream, a, cluster);
+  if (part <= 2048)
+    return launch_rows(topk_distill_kernel<T, 128, true>, rows, cluster, 128, bytes, stream, a, cluster);
+  if (part <= 4097)
+    return launch_rows(topk_distill_kernel<T, 256, true>, rows, cluster, 256, bytes, stream, a, cluster);
+  return launch_rows(topk_distill_kernel<T, 512, true>, rows, cluster, 512, bytes, stream, a, cluster);
 }
 
 }  // namespace

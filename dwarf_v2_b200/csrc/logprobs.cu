@@ -231,9 +231,9 @@ __global__ void __launch_bounds__(kRowThreads, 9)
   const Part<T> part(x, vocab, rank, cluster);
   Sums sum = {-CUDART_INF_F, 0.0f, 0.0f};
   float top0 = -CUDART_INF_F, top1 = -CUDART_INF_F;  // maxima of the thread's even and odd vectors
-  for (int first = part.j0; first < part.j1; first += kVectors * kRowThreads) {
+  for (int at = 0; at < part.size(); at += kVectors * kRowThreads) {
     uint4 v[kVectors];
-    part.load(first, v);
+    part.load(at, v);
     typename V::Max mv[2];
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kRowThreads, 9)
     if (kTop) {
       top0 = fmaxf(top0, V::largest(mv[0]));
       top1 = fmaxf(top1, V::largest(mv[1]));
-      typename V::Narrow* cell = s_cells + (first - part.j0) / kVectors * 2 + 2 * tid;
+      typename V::Narrow* cell = s_cells + at / kVectors * 2 + 2 * tid;
       cell[0] = V::narrow(mv[0]);
       cell[1] = V::narrow(mv[1]);
     }
@@ -274,14 +274,13 @@ __global__ void __launch_bounds__(kRowThreads, 9)
         t = fma2(p, d, t);
       }
     };
-    if (packed) {
+    if (packed && at + kVectors * kRowThreads <= part.size()) {
 #pragma unroll
-      for (int i = 0; i < kVectors; ++i)
-        if (first + i * kRowThreads < part.j1) add(V::clamp(v[i], low), false);
+      for (int i = 0; i < kVectors; ++i) add(V::clamp(v[i], low), false);
     } else {
 #pragma unroll
       for (int i = 0; i < kVectors; ++i)
-        if (first + i * kRowThreads < part.j1) add(v[i], true);
+        if (at + i * kRowThreads < part.size()) add(v[i], true);
     }
     sum.s += s.x + s.y;
     sum.t += t.x + t.y;
@@ -449,7 +448,7 @@ __global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
   const float g_h = a.g_entropy != nullptr ? a.g_entropy[r] : 0.0f;
   any = __syncthreads_or(any) || g_lse != 0.0f || g_h != 0.0f;
   if (!any || ms.y == 0.0f) {
-    for (int j = part.j0 + tid; j < part.j1; j += kRowThreads) store.zero(j);
+    for (int at = 0; at < part.size(); at += kVectors * kRowThreads) store.zero(part, at);
     return;
   }
   const float weight = off ? CUDART_NAN_F : g - g_lse;
@@ -464,19 +463,16 @@ __global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
     d = make_float2(fmaxf(d.x, -200.0f), fmaxf(d.y, -200.0f));
     return mul2(e, fma2(make_float2(k_b, k_b), d, make_float2(k_a, k_a)));
   };
-  for (int first = part.j0; first < part.j1; first += kVectors * kRowThreads) {
+  for (int at = 0; at < part.size(); at += kVectors * kRowThreads) {
     uint4 v[kVectors];
-    part.load(first, v);
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      const int j = first + i * kRowThreads + tid;
-      if (j >= part.j1) break;
+    part.load(at, v);
+    store.tile(part, at, v, [&](const uint4& w) {
       float2 e[V::kVec / 2];
-      V::unpack(v[i], e);
+      V::unpack(w, e);
 #pragma unroll
       for (int h = 0; h < V::kVec / 2; ++h) e[h] = dense(e[h]);
-      store.put(j, V::pack(e));
-    }
+      return V::pack(e);
+    });
   }
   __syncthreads();  // the listed entries are written again, with their own terms
   for (int j = tid; j < n; j += kRowThreads) {

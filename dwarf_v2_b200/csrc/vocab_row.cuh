@@ -16,8 +16,8 @@ constexpr int kMaxCluster = 8;
 
 // Row r of logits [outer, inner, vocab] with two row strides.
 __device__ __forceinline__ int64_t row_offset(int64_t r, int64_t inner, int64_t so, int64_t si) {
-  const int64_t o = r / inner;
-  return o * so + (r - o * inner) * si;
+  const uint32_t o = (uint32_t)r / (uint32_t)inner;  // fewer than 2^28 rows
+  return o * so + (int64_t)((uint32_t)r - o * (uint32_t)inner) * si;
 }
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
@@ -237,16 +237,27 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
   return v;
 }
 
-// 16 bytes into shared memory without passing through registers.
-__device__ __forceinline__ void copy16_async(void* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
-               : "memory");
+// L2 keeps lines read under the first policy while it can, and gives up those read under the second.
+__device__ __forceinline__ uint64_t policy_keep() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+  return p;
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// Waits until at most kLeft of the thread's committed groups are in flight.
-template <int kLeft>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+__device__ __forceinline__ uint64_t policy_leave() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ uint4 ld_stream(const void* p, uint64_t policy) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p), "l"(policy));
+  return v;
+}
+// Asks L2 for `bytes` (a multiple of 16) from a 16-byte boundary.
+__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes, uint64_t policy) {
+  asm volatile("cp.async.bulk.prefetch.L2.global.L2::cache_hint [%0], %1, %2;" ::"l"(p), "r"(bytes), "l"(policy)
+               : "memory");
 }
 
 __device__ __forceinline__ void st_stream(void* p, const uint4& v) {
@@ -356,12 +367,17 @@ struct Part {
     j0 = min(rank * per, n);
     j1 = min(j0 + per, n);
   }
-  // Vectors first, first + threads, ...; places outside the part as -inf.
-  __device__ __forceinline__ void load(int first, uint4 (&v)[kVectors]) const {
-    const int j = first + threadIdx.x;
-    const int lo = row.lead > 0 ? 1 : 0, hi = row.end / kVec;  // the whole vectors
-    const uint4* p = reinterpret_cast<const uint4*>(row.base) + j;
-    if (first >= lo && first + kVectors * kThreads <= min(j1, hi)) {
+  __device__ __forceinline__ int size() const { return j1 - j0; }
+  // Whether all vectors of the tile that starts `at` vectors into the part are whole: its
+  // loops then need no checks (they cost a third of the instructions of the gradient).
+  __device__ __forceinline__ bool full(int at) const {
+    return j0 + at >= (row.lead > 0 ? 1 : 0) && j0 + at + kVectors * kThreads <= min(j1, row.end / kVec);
+  }
+  // Vectors at, at + threads, ...; places outside the part as -inf.
+  __device__ __forceinline__ void load(int at, uint4 (&v)[kVectors]) const {
+    const int j = j0 + at + threadIdx.x;
+    if (full(at)) {
+      const uint4* p = reinterpret_cast<const uint4*>(row.base) + j;
 #pragma unroll
       for (int i = 0; i < kVectors; ++i) v[i] = ld_stream(p + i * kThreads);
       return;
@@ -372,14 +388,17 @@ struct Part {
       if (j + i * kThreads < j1) v[i] = row.load(j + i * kThreads);
     }
   }
-  // The same from a copy of the part.
-  __device__ __forceinline__ void load_from(const uint4* kept, int first, uint4 (&v)[kVectors]) const {
-    const int j = first - j0 + threadIdx.x;
+  // The same under an L2 policy.
+  __device__ __forceinline__ void load(int at, uint4 (&v)[kVectors], uint64_t policy) const {
+    if (!full(at)) return load(at, v);
+    const uint4* p = reinterpret_cast<const uint4*>(row.base) + (j0 + at + threadIdx.x);
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      v[i] = make_uint4(Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf);
-      if (j + i * kThreads < j1 - j0) v[i] = kept[j + i * kThreads];
-    }
+    for (int i = 0; i < kVectors; ++i) v[i] = ld_stream(p + i * kThreads, policy);
+  }
+  // Asks L2 for the part's whole vectors; by one thread.
+  __device__ __forceinline__ void prefetch(uint64_t policy) const {
+    const int lo = max(j0, row.lead > 0 ? 1 : 0), hi = min(j1, row.end / kVec);
+    if (lo < hi) prefetch_l2(reinterpret_cast<const uint4*>(row.base) + lo, (uint32_t)(hi - lo) * 16u, policy);
   }
   __device__ __forceinline__ bool holds(int id) const {
     const int j = (id + row.lead) / kVec;
@@ -431,7 +450,25 @@ struct RowStore {
       if (u >= row.lead && u < row.end) out[u - row.lead] = e[i];
     }
   }
-  __device__ __forceinline__ void zero(int j) const { put(j, make_uint4(0, 0, 0, 0)); }
+  // f of each vector of a tile of `part`, stored.
+  template <int kThreads, typename F>
+  __device__ __forceinline__ void tile(const Part<T, kThreads>& part, int at, const uint4 (&v)[kVectors], F f) const {
+    const int j = part.j0 + at + threadIdx.x;
+    if (same && part.full(at)) {
+      T* o = out + ((int64_t)j * kVec - row.lead);
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) st_stream(o + i * kThreads * kVec, f(v[i]));
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+      if (j + i * kThreads < part.j1) put(j + i * kThreads, f(v[i]));
+  }
+  template <int kThreads>
+  __device__ __forceinline__ void zero(const Part<T, kThreads>& part, int at) const {
+    const uint4 v[kVectors] = {};
+    tile(part, at, v, [](const uint4& w) { return w; });
+  }
 };
 
 // How many CTAs share a row: more than one only while the rows alone leave SMs with
