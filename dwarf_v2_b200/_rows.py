@@ -39,6 +39,8 @@ def same_device(logits: torch.Tensor, **others: torch.Tensor | None) -> None:
 
 def ids64(t: torch.Tensor, shape, name: str) -> torch.Tensor:
     """A contiguous int64 tensor of ``shape``."""
+    if t.dtype is torch.int64 and t.shape == shape and t.is_contiguous():
+        return t
     if t.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"{name} must be int64 or int32, got {t.dtype}")
     if tuple(t.shape) != tuple(shape):
@@ -53,6 +55,9 @@ def addressed(logits: torch.Tensor) -> tuple[torch.Tensor, int, int, int, int]:
     (``logits[:, :-1]``) are read in place, anything else is copied first."""
     if logits.stride(-1) != 1 and logits.shape[-1] > 1:
         logits = logits.contiguous()
+    if logits.is_contiguous():
+        vocab = logits.shape[-1]
+        return logits, 1, logits.numel() // vocab, 0, vocab
     groups: list[list[int]] = []
     for n, stride in zip(logits.shape[:-1], logits.stride()[:-1]):
         if n == 1:

@@ -11,6 +11,7 @@ namespace dwarf {
 namespace {
 
 constexpr int kGroups = 2 * kRowThreads;
+constexpr int kCells = 4;           // cells that the vectors of a thread's tile fall into
 constexpr int kCandidates = 512;    // entries that the search for the alternatives sorts
 constexpr int kHits = 512;          // cells that it looks through
 
@@ -31,21 +32,49 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
 }
 
-// How many of the n keys are above `key`.
-__device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int n) {
-  int above = 0;
-  const ulonglong2* q = reinterpret_cast<const ulonglong2*>(keys);
-#pragma unroll 4
-  for (int i = 0; i < n / 2; ++i) {
-    const ulonglong2 w = q[i];
-    above += (w.x > key) + (w.y > key);
+// Sorts a warp's keys, the largest in lane 0: a bitonic network of 15 steps.
+__device__ __forceinline__ uint64_t warp_sort(uint64_t key) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2) {
+#pragma unroll
+    for (int o = size / 2; o >= 1; o /= 2) {
+      const uint64_t other = __shfl_xor_sync(0xffffffffu, key, o);
+      const bool larger = ((lane & size) == 0) == ((lane & o) == 0);  // this lane keeps the larger
+      if ((other > key) == larger) key = other;
+    }
   }
-  if (n & 1) above += keys[n - 1] > key;
-  return above;
+  return key;
+}
+
+// f(key, rank) for the n keys (all unlike; none is 0): runs of 32 are sorted by a warp each,
+// a key's rank in the other runs is searched. (A rank by comparison with all n keys takes
+// n^2 / 32 steps: 890 for the 177 candidates of 128 entries, against about 350.) Of the whole block.
+template <typename F>
+__device__ __forceinline__ void for_ranked(uint64_t* keys, int n, F f) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int c = 32 * warp; c < n; c += kRowThreads) {
+    const uint64_t key = warp_sort(c + lane < n ? keys[c + lane] : 0);
+    keys[c + lane] = key;
+  }
+  __syncthreads();
+  for (int c = 32 * warp; c < n; c += kRowThreads) {
+    const uint64_t key = keys[c + lane];
+    int above = lane;
+    for (int o = 0; o < n; o += 32) {
+      if (o == c) continue;
+      int at = o;  // entries of the run from o on that are above the key
+#pragma unroll
+      for (int step = 16; step >= 1; step /= 2)
+        if (keys[at + step - 1] > key) at += step;
+      above += at - o + (keys[at] > key);
+    }
+    if (key != 0) f(key, above);
+  }
 }
 
 struct TopShared {
-  uint32_t value[kGroups];           // order keys of the maxima, two of each thread
+  uint4 value[kGroups / 8];          // the groups' maxima in 16 bits
   int hit[kHits];                    // cells that reach the bound
   alignas(16) uint64_t candidate[kCandidates];
   uint32_t bound;
@@ -53,52 +82,29 @@ struct TopShared {
   int scan[kRowThreads / 32];
 };
 
-// The smallest of the group maxima that the K-th largest 16-bit prefix among them takes in;
-// one warp, kPer groups a lane. The search starts below the bits that all groups share.
-template <int kPer>
-__device__ __forceinline__ uint32_t bound_of(const uint32_t (&g)[kPer], int k) {
-  uint32_t high = g[0], low = g[0];
-#pragma unroll
-  for (int i = 1; i < kPer; ++i) high = max(high, g[i]), low = min(low, g[i]);
-  high = __reduce_max_sync(0xffffffffu, high);
-  low = __reduce_min_sync(0xffffffffu, low);
-  const uint32_t free = high == low ? 0u : 0xffffffffu >> __clz(high ^ low);  // the bits that differ, and all below
-  uint32_t prefix = high & ~free;
-  for (uint32_t bit = free ^ (free >> 1); bit >= 0x10000u; bit >>= 1) {
-    int c = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) c += g[i] >= (prefix | bit);
-    if (__reduce_add_sync(0xffffffffu, c) >= k) prefix |= bit;
+// A bound that K entries of the part reach: the K-th largest of the maxima of G >= 2 K
+// groups of entries (K <= G suffices). With entries in random places about G ln(G / (G - K))
+// reach it. It is the smallest maximum that fewer than K exceed; each thread counts for
+// its own, in packed 16-bit pairs (a search bit by bit in one warp has a third of the
+// instructions, but its steps wait for one another: 3400 cycles against 1200 at K = 64).
+template <typename N>
+__device__ __forceinline__ void bound_of_groups(const N* value, int groups, int k, uint32_t* bound) {
+  using V = Vec16<N>;
+  for (int t = threadIdx.x; t < groups; t += kRowThreads) {
+    const N g = value[t];
+    const uint32_t zero = 0;
+    typename V::Max c = *reinterpret_cast<const typename V::Max*>(&zero);
+#pragma unroll 4
+    for (int i = 0; i < groups; i += 8) c = V::above(*reinterpret_cast<const uint4*>(value + i), g, c);
+    const uint32_t key = V::total(c) < k ? order_key(to_f32(g)) : 0xffffffffu;
+    const uint32_t least = __reduce_min_sync(0xffffffffu, key);
+    if ((threadIdx.x & 31) == 0 && least != 0xffffffffu) atomicMin(bound, least);
   }
-  uint32_t least = 0xffffffffu;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (g[i] >= prefix) least = min(least, g[i]);
-  return __reduce_min_sync(0xffffffffu, least);
-}
-
-// A bound that K entries of the part reach, from the maxima of G >= 2 K groups (K <= G suffices):
-// with entries in random places about G ln(G / (G - K)) reach it.
-__device__ __forceinline__ uint32_t bound_of_groups(const uint32_t* value, int k) {
-  const int lane = threadIdx.x & 31;
-  uint32_t g8[8], g4[4], g2[2], g1[1];
-  static_assert(kGroups == 256, "eight groups a lane");
-#pragma unroll
-  for (int i = 0; i < 8; ++i) g8[i] = value[lane + 32 * i];
-  if (k > 64) return bound_of<8>(g8, k);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) g4[i] = max(g8[i], g8[i + 4]);
-  if (k > 32) return bound_of<4>(g4, k);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) g2[i] = max(g4[i], g4[i + 2]);
-  if (k > 16) return bound_of<2>(g2, k);
-  g1[0] = max(g2[0], g2[1]);
-  return bound_of<1>(g1, k);
 }
 
 // The K best entries of the part (order: value, then lowest id) among the first n
 // candidates, n >= min(K, entries of the part). `cells` holds 16 bits, no lower than the
-// largest entry, for each cell: the even or the odd ones of a thread's vectors of a tile. The cells
+// largest entry, for each cell: every fourth of a thread's vectors of a tile. The cells
 // that reach the bound are read again (from L2) and their entries that reach it become
 // candidates. Where these are more than the buffers hold (ties, or many large values in
 // one group), or a NaN is in the row, the K-th value is found bit by bit over the whole
@@ -111,10 +117,11 @@ __device__ __forceinline__ int best_entries(const Part<T>& part, const typename 
   uint32_t limit = sh.bound;
   if (!nan) {
     const float bound = key_value(limit);
-    const int n = ceil_div(part.j1 - part.j0, kVectors * kRowThreads) * kGroups;
-    for (int c = 8 * tid; c < n; c += 8 * kRowThreads) {
-      const uint4 w = *reinterpret_cast<const uint4*>(cells + c);
-      for (uint32_t m = N16::reach(w, bound); m != 0; m &= m - 1) {
+    const int n = ceil_div(part.size(), kVectors * kRowThreads) * kCells * kRowThreads;
+    for (int first = 0; first < n; first += 8 * kRowThreads) {  // eight cells a thread
+      const int c = first + 8 * tid;
+      uint32_t m = c < n ? N16::reach(*reinterpret_cast<const uint4*>(cells + c), bound) : 0u;
+      for (; m != 0; m &= m - 1) {
         const int at = atomicAdd(&sh.hits, 1);
         if (at < kHits) sh.hit[at] = c + N16::element(__ffs(m) - 1);
       }
@@ -122,17 +129,46 @@ __device__ __forceinline__ int best_entries(const Part<T>& part, const typename 
     __syncthreads();
     const int hits = sh.hits;
     if (hits <= kHits) {
-      constexpr int kCell = kVectors / 2;
-      for (int h = tid; h < hits * kCell; h += kRowThreads) {
-        const int c = sh.hit[h / kCell];  // [tile][thread][even, odd]
-        const int j = part.j0 + (c / kGroups * kVectors + 2 * (h % kCell) + (c & 1)) * kRowThreads + (c % kGroups) / 2;
-        if (j >= part.j1) continue;
-        const uint4 w = part.row.load(j);
-        for (uint32_t m = Vec16<T>::reach(w, bound); m != 0; m &= m - 1) {
-          const int e = Vec16<T>::element(__ffs(m) - 1), u = j * Part<T>::kVec + e;
-          if (u < part.row.lead || u >= part.row.end) continue;
-          const int at = atomicAdd(&sh.n, 1);
-          if (at < kCandidates) sh.candidate[at] = entry_key(Vec16<T>::value(w, e), (uint32_t)(u - part.row.lead));
+      constexpr int kCell = kVectors / kCells, kBatch = 2;
+      const int items = hits * kCell;
+      for (int first = 0; first < items; first += kBatch * kRowThreads) {
+        uint4 w[kBatch];
+        int at_j[kBatch], found = 0;
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q) {  // the loads of a batch are in flight together
+          const int h = first + q * kRowThreads + tid;
+          at_j[q] = part.j1;
+          if (h < items) {
+            const int c = sh.hit[h / kCell];  // [tile][thread][cell]
+            at_j[q] = part.j0 + (c / (kCells * kRowThreads) * kVectors + h % kCell * kCells + c % kCells) * kRowThreads +
+                      c / kCells % kRowThreads;
+          }
+          if (at_j[q] < part.j1) w[q] = part.row.load(at_j[q]);
+        }
+        uint32_t m[kBatch];
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q) {
+          m[q] = 0;
+          if (at_j[q] >= part.j1) continue;
+          m[q] = Vec16<T>::reach(w[q], bound);
+          if (m[q] != 0 && !part.row.whole(at_j[q])) {
+            for (uint32_t all = m[q]; all != 0; all &= all - 1) {
+              const int bit = __ffs(all) - 1, u = at_j[q] * Part<T>::kVec + Vec16<T>::element(bit);
+              if (u < part.row.lead || u >= part.row.end) m[q] &= ~(1u << bit);
+            }
+          }
+          found += __popc(m[q]);
+        }
+        if (found == 0) continue;
+        int at = atomicAdd(&sh.n, found);
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q) {
+          for (; m[q] != 0; m[q] &= m[q] - 1, ++at) {
+            const int e = Vec16<T>::element(__ffs(m[q]) - 1);
+            if (at < kCandidates)
+              sh.candidate[at] = entry_key(Vec16<T>::value(w[q], e),
+                                           (uint32_t)(at_j[q] * Part<T>::kVec + e - part.row.lead));
+          }
         }
       }
       __syncthreads();
@@ -208,7 +244,7 @@ __device__ __forceinline__ int best_entries(const Part<T>& part, const typename 
 // another's sums and search; 512 threads that hold a whole row reached 4.0 of these
 // 6.4 TB/s (16384 rows of 32768 bf16, no alternatives).
 template <typename T, bool kTop>
-__global__ void __launch_bounds__(kRowThreads, 9)
+__global__ void __launch_bounds__(kRowThreads, kTop ? 9 : 8)
     token_logprobs_kernel(const dwarf_token_logprobs_args a, int cluster, int lists_at) {
   using V = Vec16<T>;
   constexpr int kWarps = kRowThreads / 32;
@@ -230,24 +266,29 @@ __global__ void __launch_bounds__(kRowThreads, 9)
 
   const Part<T> part(x, vocab, rank, cluster);
   Sums sum = {-CUDART_INF_F, 0.0f, 0.0f};
-  float top0 = -CUDART_INF_F, top1 = -CUDART_INF_F;  // maxima of the thread's even and odd vectors
+  typename V::Max top0 = V::none(), top1 = V::none();  // maxima of the thread's even and odd vectors
   for (int at = 0; at < part.size(); at += kVectors * kRowThreads) {
     uint4 v[kVectors];
     part.load(at, v);
-    typename V::Max mv[2];
+    typename V::Max mv[kCells];
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
       const typename V::Max of = V::max_of(v[i]);
-      mv[i & 1] = i < 2 ? of : V::join(mv[i & 1], of);
+      mv[i % kCells] = i < kCells ? of : V::join(mv[i % kCells], of);
+    }
+    if (kTop) {
+      __align__(8) typename V::Narrow cell[kCells];
+#pragma unroll
+      for (int i = 0; i < kCells; ++i) cell[i] = V::narrow(mv[i]);
+      reinterpret_cast<uint2*>(s_cells)[at / kVectors + tid] = *reinterpret_cast<const uint2*>(cell);
+    }
+    mv[0] = V::join(mv[0], mv[2]);
+    mv[1] = V::join(mv[1], mv[3]);
+    if (kTop) {
+      top0 = V::join(top0, mv[0]);
+      top1 = V::join(top1, mv[1]);
     }
     const float mx = V::largest(V::join(mv[0], mv[1]));
-    if (kTop) {
-      top0 = fmaxf(top0, V::largest(mv[0]));
-      top1 = fmaxf(top1, V::largest(mv[1]));
-      typename V::Narrow* cell = s_cells + at / kVectors * 2 + 2 * tid;
-      cell[0] = V::narrow(mv[0]);
-      cell[1] = V::narrow(mv[1]);
-    }
     const float m = fmaxf(sum.m, warp_max(mx));
     if (sum.m > -CUDART_INF_F) {  // a later tile: move the sums to the new maximum
       const float d = fmaxf((sum.m - m) * c2, -200.0f), f = ex2_approx(d);
@@ -255,32 +296,48 @@ __global__ void __launch_bounds__(kRowThreads, 9)
       sum.s *= f;
     }
     sum.m = m;
-    const float shift = m == -CUDART_INF_F ? 0.0f : -m;
     float2 s = make_float2(0.0f, 0.0f), t = s;
     // Entries 2^-200 below the maximum count as 0, masked ones among them (0 (-inf) is
-    // not formed). The bound is set in the row's type where that has room for it below
-    // the maximum (2^-60 at least), in fp32 otherwise.
+    // not formed). Where the row's type has room for such a bound below the maximum
+    // (2^-60 at least) and c m is no extreme value, the bound is set in packed pairs and
+    // d = c x - c m takes one fused operation; what the rounding of c m leaves out is put
+    // back into the sums. Otherwise d = c (x - m) and the bound is set in fp32.
     const typename V::Low low = V::low_of(m - 200.0f / c2);
-    const bool packed = (m - V::low_value(low)) * c2 >= 60.0f && V::low_value(low) > -1.0e38f;
-    auto add = [&](const uint4& w, bool clamp) {
+    const float cm = m * c2;
+    if ((m - V::low_value(low)) * c2 >= 60.0f && fabsf(cm) < 1.0e30f && at + kVectors * kRowThreads <= part.size()) {
+      const float2 shift = make_float2(-cm, -cm), cc = make_float2(c2, c2);
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) {
+        float2 e[V::kVec / 2];
+        V::unpack(V::clamp(v[i], low), e);
+#pragma unroll
+        for (int h = 0; h < V::kVec / 2; ++h) {
+          const float2 d = fma2(e[h], cc, shift);
+          const float2 p = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+          s = add2(s, p);
+          t = fma2(p, d, t);
+        }
+      }
+      const float left = fmaf(m, c2, -cm), f = ex2_approx(-left);
+      const float s1 = s.x + s.y;
+      sum.s += f * s1;
+      sum.t += f * fmaf(-left, s1, t.x + t.y);
+      continue;
+    }
+    const float shift = m == -CUDART_INF_F ? 0.0f : -m;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+      if (at + i * kRowThreads >= part.size()) break;
       float2 e[V::kVec / 2];
-      V::unpack(w, e);
+      V::unpack(v[i], e);
 #pragma unroll
       for (int h = 0; h < V::kVec / 2; ++h) {
         float2 d = mul2(add2(e[h], make_float2(shift, shift)), make_float2(c2, c2));
         const float2 p = make_float2(ex2_approx(d.x), ex2_approx(d.y));
-        if (clamp) d = make_float2(fmaxf(d.x, -200.0f), fmaxf(d.y, -200.0f));
+        d = make_float2(fmaxf(d.x, -200.0f), fmaxf(d.y, -200.0f));
         s = add2(s, p);
         t = fma2(p, d, t);
       }
-    };
-    if (packed && at + kVectors * kRowThreads <= part.size()) {
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i) add(V::clamp(v[i], low), false);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i)
-        if (at + i * kRowThreads < part.size()) add(v[i], true);
     }
     sum.s += s.x + s.y;
     sum.t += t.x + t.y;
@@ -288,10 +345,21 @@ __global__ void __launch_bounds__(kRowThreads, 9)
   sum.s = warp_sum(sum.s);
   sum.t = warp_sum(sum.t);
   if (lane == 0) s_warp[warp] = sum;
+  int groups = 0;
   if (kTop) {
-    top.value[tid] = order_key(top0);
-    top.value[kRowThreads + tid] = order_key(top1);
-    if (tid == 0) top.n = top.hits = 0;
+    typename V::Narrow* value = reinterpret_cast<typename V::Narrow*>(top.value);
+    if (k > 64) {
+      value[tid] = V::narrow_down(top0);
+      value[kRowThreads + tid] = V::narrow_down(top1);
+      groups = 2 * kRowThreads;
+    } else {
+      top0 = V::join(top0, top1);
+      int each = 32;  // groups of a warp
+      for (; each > 8 && k * 4 <= each * kWarps; each /= 2) top0 = V::join(top0, __shfl_xor_sync(0xffffffffu, top0, each / 2));
+      if (lane < each) value[warp * each + lane] = V::narrow_down(top0);
+      groups = each * kWarps;
+    }
+    if (tid == 0) top.n = top.hits = 0, top.bound = 0xffffffffu;
   }
   __syncthreads();
   if (cluster > 1) cluster_wait();
@@ -307,10 +375,7 @@ __global__ void __launch_bounds__(kRowThreads, 9)
   }
   int n = 0;
   if (kTop) {
-    if (warp == 0) {
-      const uint32_t bound = bound_of_groups(top.value, k);
-      if (lane == 0) top.bound = bound;
-    }
+    bound_of_groups(reinterpret_cast<const typename V::Narrow*>(top.value), groups, k, &top.bound);
     __syncthreads();
     // a NaN or +inf anywhere in the part makes some warp's sum NaN
     bool nan = false;
@@ -320,15 +385,11 @@ __global__ void __launch_bounds__(kRowThreads, 9)
   }
   if (cluster > 1) {
     if (kTop) {
-      for (int c = tid; c < max(n, k); c += kRowThreads) {
-        uint64_t key = 0;
-        int at = c;
-        if (c < n) {
-          key = top.candidate[c];
-          at = rank_of(key, top.candidate, n);
-        }
+      auto send = [&](uint64_t key, int at) {
         if (at < k) st_cluster(cluster_address(&s_lists[rank * k + at], 0), key);
-      }
+      };
+      for_ranked(top.candidate, n, send);
+      for (int at = n + tid; at < k; at += kRowThreads) send(0, at);
     }
     cluster_arrive();
     if (rank != 0) return;
@@ -369,11 +430,9 @@ __global__ void __launch_bounds__(kRowThreads, 9)
         fin.s == 0.0f ? -CUDART_INF_F : (key_value((uint32_t)(key >> 32)) - fin.m) * a.inv_temperature - fin.t;
   };
   if (cluster == 1) {
-    for (int c = tid; c < n; c += kRowThreads) {
-      const uint64_t key = top.candidate[c];
-      const int at = rank_of(key, top.candidate, n);
+    for_ranked(top.candidate, n, [&](uint64_t key, int at) {
       if (at < k) put(key, at);
-    }
+    });
   } else {
     for (int c = tid; c < cluster * k; c += kRowThreads) {
       const uint64_t key = s_lists[c];
@@ -397,11 +456,11 @@ template <typename T>
 int launch_forward(const dwarf_token_logprobs_args& a, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner;
   const int vectors = ceil_div((int)a.vocab, Vec16<T>::kVec);
-  const int cluster = cluster_for(rows, vectors, 65536);  // cells: at most 32 KB
+  const int cluster = cluster_for(rows, vectors, 65536);  // cells: at most 64 KB
   if (a.top_k == 0)
     return launch_rows(token_logprobs_kernel<T, false>, rows, cluster, kRowThreads, 0, stream, a, cluster, 0);
   // a row that starts off a 16-byte boundary has one vector more
-  const int lists_at = ceil_div(ceil_div(vectors + 1, cluster), kVectors * kRowThreads) * kGroups * 2;
+  const int lists_at = ceil_div(ceil_div(vectors + 1, cluster), kVectors * kRowThreads) * kCells * kRowThreads * 2;
   const int bytes = lists_at + (cluster > 1 ? cluster * a.top_k * 8 : 0);
   const auto kernel = token_logprobs_kernel<T, true>;
   if (bytes > 32 * 1024 &&

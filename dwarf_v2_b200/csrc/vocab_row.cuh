@@ -96,9 +96,11 @@ struct Vec16<float> {
     return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
   }
   __device__ __forceinline__ static Max join(Max a, Max b) { return fmaxf(a, b); }
+  __device__ __forceinline__ static Max none() { return -CUDART_INF_F; }
   __device__ __forceinline__ static float largest(Max a) { return a; }
-  using Narrow = __nv_bfloat16;  // 16 bits that are no lower than the largest
+  using Narrow = __nv_bfloat16;  // 16 bits that are no lower than the largest, and no higher
   __device__ __forceinline__ static Narrow narrow(Max a) { return __float2bfloat16_ru(a); }
+  __device__ __forceinline__ static Narrow narrow_down(Max a) { return __float2bfloat16_rd(a); }
   // The elements of at least `bound` (the nearest lower value of the type) as bits; the element of a bit; its value.
   __device__ __forceinline__ static uint32_t reach(const uint4& v, float bound) {
     return (uint32_t)(__uint_as_float(v.x) >= bound) | (uint32_t)(__uint_as_float(v.y) >= bound) << 1 |
@@ -143,11 +145,16 @@ struct Vec16<__nv_bfloat16> {
   using Max = __nv_bfloat162;
   using Narrow = __nv_bfloat16;
   __device__ __forceinline__ static Narrow narrow(Max a) { return __hmax(__low2bfloat16(a), __high2bfloat16(a)); }
+  __device__ __forceinline__ static Narrow narrow_down(Max a) { return narrow(a); }
   __device__ __forceinline__ static Max max_of(const uint4& v) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
     return __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
   }
   __device__ __forceinline__ static Max join(Max a, Max b) { return __hmax2(a, b); }
+  __device__ __forceinline__ static Max none() {
+    const uint32_t w = kMinusInf;
+    return *reinterpret_cast<const Max*>(&w);
+  }
   __device__ __forceinline__ static float largest(Max a) {
     const float2 f = __bfloat1622float2(a);
     return fmaxf(f.x, f.y);
@@ -157,6 +164,19 @@ struct Vec16<__nv_bfloat16> {
     const __nv_bfloat162 b = __bfloat162bfloat162(__float2bfloat16_rd(bound));
     return (__hge2_mask(h[0], b) & 0x00010001u) | (__hge2_mask(h[1], b) & 0x00020002u) |
            (__hge2_mask(h[2], b) & 0x00040004u) | (__hge2_mask(h[3], b) & 0x00080008u);
+  }
+  // Adds the places' numbers of elements above g to c (exact up to 256).
+  __device__ __forceinline__ static __nv_bfloat162 above(const uint4& v, __nv_bfloat16 g, __nv_bfloat162 c) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const __nv_bfloat162 b = __bfloat162bfloat162(g);
+    c = __hadd2(c, __hgt2(h[0], b));
+    c = __hadd2(c, __hgt2(h[1], b));
+    c = __hadd2(c, __hgt2(h[2], b));
+    return __hadd2(c, __hgt2(h[3], b));
+  }
+  __device__ __forceinline__ static int total(__nv_bfloat162 c) {
+    const float2 f = __bfloat1622float2(c);
+    return (int)(f.x + f.y);
   }
   __device__ __forceinline__ static int element(int bit) { return 2 * (bit & 15) + (bit >> 4); }
   __device__ __forceinline__ static float value(const uint4& v, int e) {
@@ -197,11 +217,16 @@ struct Vec16<__half> {
   using Max = __half2;
   using Narrow = __half;
   __device__ __forceinline__ static Narrow narrow(Max a) { return __hmax(__low2half(a), __high2half(a)); }
+  __device__ __forceinline__ static Narrow narrow_down(Max a) { return narrow(a); }
   __device__ __forceinline__ static Max max_of(const uint4& v) {
     const __half2* h = reinterpret_cast<const __half2*>(&v);
     return __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
   }
   __device__ __forceinline__ static Max join(Max a, Max b) { return __hmax2(a, b); }
+  __device__ __forceinline__ static Max none() {
+    const uint32_t w = kMinusInf;
+    return *reinterpret_cast<const Max*>(&w);
+  }
   __device__ __forceinline__ static float largest(Max a) {
     const float2 f = __half22float2(a);
     return fmaxf(f.x, f.y);
@@ -211,6 +236,19 @@ struct Vec16<__half> {
     const __half2 b = __half2half2(__float2half_rd(bound));
     return (__hge2_mask(h[0], b) & 0x00010001u) | (__hge2_mask(h[1], b) & 0x00020002u) |
            (__hge2_mask(h[2], b) & 0x00040004u) | (__hge2_mask(h[3], b) & 0x00080008u);
+  }
+  // Adds the places' numbers of elements above g to c (exact up to 256).
+  __device__ __forceinline__ static __half2 above(const uint4& v, __half g, __half2 c) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    const __half2 b = __half2half2(g);
+    c = __hadd2(c, __hgt2(h[0], b));
+    c = __hadd2(c, __hgt2(h[1], b));
+    c = __hadd2(c, __hgt2(h[2], b));
+    return __hadd2(c, __hgt2(h[3], b));
+  }
+  __device__ __forceinline__ static int total(__half2 c) {
+    const float2 f = __half22float2(c);
+    return (int)(f.x + f.y);
   }
   __device__ __forceinline__ static int element(int bit) { return 2 * (bit & 15) + (bit >> 4); }
   __device__ __forceinline__ static float value(const uint4& v, int e) {

@@ -35,12 +35,17 @@ def _forward(logits: torch.Tensor, targets: torch.Tensor | None, top_k: int, inv
              ignore_index: int, want_stats: bool):
     dev, lead = logits.device, logits.shape[:-1]
     logits, outer, inner, so, si = _rows.addressed(logits)
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+    if targets is None:
+        logprob, entropy = None, torch.empty(lead, dtype=torch.float32, device=dev)
+    else:
+        logprob = torch.empty_like(targets, dtype=torch.float32)
+        entropy = torch.empty_like(logprob)
     lse = torch.empty_like(entropy)
-    logprob = None if targets is None else torch.empty_like(entropy)
     stats = torch.empty(*lead, 2, dtype=torch.float32, device=dev) if want_stats else None
-    top_logprobs = torch.empty(*lead, top_k, dtype=torch.float32, device=dev) if top_k else None
-    top_ids = torch.empty(*lead, top_k, dtype=torch.int64, device=dev) if top_k else None
+    top_logprobs = top_ids = None
+    if top_k:
+        top_logprobs = torch.empty(*lead, top_k, dtype=torch.float32, device=dev)
+        top_ids = torch.empty_like(top_logprobs, dtype=torch.int64)
     args = _lib.TokenLogprobsArgs(
         version=_lib.ABI_VERSION, dtype=_lib.dtype_code(logits.dtype), logits=logits.data_ptr(), outer=outer,
         inner=inner, vocab=logits.shape[-1], so=so, si=si, targets=_lib.ptr(targets), ignore_index=ignore_index,
