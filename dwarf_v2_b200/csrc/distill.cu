@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_kernel(const dwarf
 
   // the teacher's slots, one a thread
   const bool counted = a.row_mask == nullptr || a.row_mask[r] != 0;
-  if (kGrad && tid == 0 && counted) part.prefetch(keep);
+  if (kGrad && tid == 0 && counted) part.prefetch_kept(keep);
   int id = -1;  // not used; vocab: past the vocabulary
   float l = -CUDART_INF_F;
   if (tid < k && counted) {

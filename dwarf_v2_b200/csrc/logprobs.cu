@@ -243,9 +243,9 @@ __device__ __forceinline__ int best_entries(const Part<T>& part, const typename 
 // and T for each warp. Eight CTAs of 128 threads on an SM overlap one's loads with
 // another's sums and search; 512 threads that hold a whole row reached 4.0 of these
 // 6.4 TB/s (16384 rows of 32768 bf16, no alternatives).
-template <typename T, bool kTop>
+template <typename T, bool kTop, bool kAhead>
 __global__ void __launch_bounds__(kRowThreads, kTop ? 9 : 8)
-    token_logprobs_kernel(const dwarf_token_logprobs_args a, int cluster, int lists_at) {
+    token_logprobs_kernel(const dwarf_token_logprobs_args a, int cluster, int lists_at, int64_t ahead) {
   using V = Vec16<T>;
   constexpr int kWarps = kRowThreads / 32;
   extern __shared__ __align__(16) unsigned char s_dynamic[];
@@ -342,6 +342,13 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 9 : 8)
     sum.s += s.x + s.y;
     sum.t += t.x + t.y;
   }
+  // The next wave's row begins to arrive in L2 while this one's tail runs. In few waves the
+  // tails leave memory idle (2047 rows of 32768 bf16, 5 alternatives: 37.0 us without, 34.9
+  // with; 4096 of fp32: 94.6, 86.5); in many the CTAs have drifted apart, and only rows
+  // without a search for alternatives still gain (16384 rows: 166 without, 162 with; with 64
+  // alternatives: 217 without, 228 with).
+  if (kAhead && tid == 0 && r + ahead < a.outer * a.inner)
+    Part<T>(static_cast<const T*>(a.logits) + row_offset(r + ahead, a.inner, a.so, a.si), vocab, 0, 1).prefetch_first(2048);
   sum.s = warp_sum(sum.s);
   sum.t = warp_sum(sum.t);
   if (lane == 0) s_warp[warp] = sum;
@@ -457,16 +464,17 @@ int launch_forward(const dwarf_token_logprobs_args& a, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner;
   const int vectors = ceil_div((int)a.vocab, Vec16<T>::kVec);
   const int cluster = cluster_for(rows, vectors, 65536);  // cells: at most 64 KB
+  const int64_t wave = cluster > 1 ? rows : (a.top_k > 0 ? 9 : 8) * kNumSMs;  // rows in flight
   if (a.top_k == 0)
-    return launch_rows(token_logprobs_kernel<T, false>, rows, cluster, kRowThreads, 0, stream, a, cluster, 0);
+    return launch_rows(token_logprobs_kernel<T, false, true>, rows, cluster, kRowThreads, 0, stream, a, cluster, 0, wave);
   // a row that starts off a 16-byte boundary has one vector more
   const int lists_at = ceil_div(ceil_div(vectors + 1, cluster), kVectors * kRowThreads) * kCells * kRowThreads * 2;
   const int bytes = lists_at + (cluster > 1 ? cluster * a.top_k * 8 : 0);
-  const auto kernel = token_logprobs_kernel<T, true>;
+  const auto kernel = rows <= 4 * wave ? token_logprobs_kernel<T, true, true> : token_logprobs_kernel<T, true, false>;
   if (bytes > 32 * 1024 &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
     return launch_status();
-  return launch_rows(kernel, rows, cluster, kRowThreads, bytes, stream, a, cluster, lists_at);
+  return launch_rows(kernel, rows, cluster, kRowThreads, bytes, stream, a, cluster, lists_at, wave);
 }
 
 // grad_v = c (sparse terms - q_v (G + gH (log q_v + H))): each CTA writes its part of the

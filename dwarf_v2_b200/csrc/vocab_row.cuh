@@ -298,6 +298,10 @@ __device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes, uint6
                : "memory");
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+
 __device__ __forceinline__ void st_stream(void* p, const uint4& v) {
   asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                : "memory");
@@ -433,10 +437,14 @@ struct Part {
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) v[i] = ld_stream(p + i * kThreads, policy);
   }
-  // Asks L2 for the part's whole vectors; by one thread.
-  __device__ __forceinline__ void prefetch(uint64_t policy) const {
+  // Asks L2 for the part's whole vectors under a policy, or for the first `most` of them; by one thread.
+  __device__ __forceinline__ void prefetch_kept(uint64_t policy) const {
     const int lo = max(j0, row.lead > 0 ? 1 : 0), hi = min(j1, row.end / kVec);
     if (lo < hi) prefetch_l2(reinterpret_cast<const uint4*>(row.base) + lo, (uint32_t)(hi - lo) * 16u, policy);
+  }
+  __device__ __forceinline__ void prefetch_first(int most) const {
+    const int lo = max(j0, row.lead > 0 ? 1 : 0), hi = min(min(j1, row.end / kVec), lo + most);
+    if (lo < hi) prefetch_l2(reinterpret_cast<const uint4*>(row.base) + lo, (uint32_t)(hi - lo) * 16u);
   }
   __device__ __forceinline__ bool holds(int id) const {
     const int j = (id + row.lead) / kVec;
