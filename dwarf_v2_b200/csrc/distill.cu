@@ -28,7 +28,7 @@ __device__ __forceinline__ void warp_join(float c2, float& m, float& a, float& b
 // without either: 534, with 475 MB read for 268; the row held in shared memory: 483; 512
 // threads: 540). The loss alone: 128 threads, no prefetch, 196 us (256 threads: 249).
 template <typename T, int NT, bool kGrad>
-__global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_kernel(const dwarf_topk_distill_args a, int cluster) {
+__device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, int cluster, int64_t r) {
   using V = Vec16<T>;
   constexpr int kWarps = NT / 32, kTile = kVectors * NT, kListWarps = DWARF_TOP_K_MAX / 32;
   static_assert(NT >= DWARF_TOP_K_MAX, "one thread for each slot of the teacher's list");
@@ -40,11 +40,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_kernel(const dwarf
   __shared__ int s_id[DWARF_TOP_K_MAX];
   __shared__ float s_p[DWARF_TOP_K_MAX];
   __shared__ int s_flags, s_listed;
-  if (a.skip_if_one && *a.grad_rows == 1.0f) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int vocab = (int)a.vocab, k = a.k;
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
-  const int64_t r = blockIdx.x / (unsigned)cluster;
   if (cluster > 1) cluster_arrive();  // its CTAs have started, before one writes to another
   const T* x = static_cast<const T*>(a.logits) + row_offset(r, a.inner, a.so, a.si);
   const Part<T, NT> part(x, vocab, rank, cluster);
@@ -141,9 +139,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_kernel(const dwarf
         add(v[i], (bits[i * NT * V::kVec / 8] >> bits_shift) & ((1u << V::kVec) - 1u));
     } else {
 #pragma unroll
-      for (int i = 0; i < kVectors; ++i)
-        if (at + i * NT + tid < part.size())
-          add(v[i], (bits[i * NT * V::kVec / 8] >> bits_shift) & ((1u << V::kVec) - 1u));
+      for (int i = 0; i < kVectors; ++i) {
+        if (at + i * NT >= part.size()) break;
+        const bool in = at + i * NT + tid < part.size();  // vectors outside hold -inf
+        add(v[i], in ? (bits[i * NT * V::kVec / 8] >> bits_shift) & ((1u << V::kVec) - 1u) : 0u);
+      }
     }
   }
   float s_r = warp_sum(sum.x + sum.y), s_l = warp_sum(sum_list.x + sum_list.y);
@@ -240,6 +240,23 @@ __global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_kernel(const dwarf
   }
 }
 
+template <typename T, int NT, bool kGrad>
+__global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_kernel(const dwarf_topk_distill_args a, int cluster) {
+  if (a.skip_if_one && *a.grad_rows == 1.0f) return;
+  distill_row<T, NT, kGrad>(a, cluster, blockIdx.x / (unsigned)cluster);
+}
+
+// The gradient anew where the upstream gradient is not 1: a grid of one wave, which costs 3 us
+// (a CTA for each of 16384 rows: 11 us) where there is nothing to do.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_again_kernel(const dwarf_topk_distill_args a) {
+  if (*a.grad_rows == 1.0f) return;
+  for (int64_t r = blockIdx.x; r < a.outer * a.inner; r += gridDim.x) {
+    distill_row<T, NT, true>(a, 1, r);
+    __syncthreads();  // before the next row's list takes this one's place
+  }
+}
+
 __global__ void __launch_bounds__(1024) row_reduce_kernel(dwarf_row_reduce_args a) {
   __shared__ double sd[32];
   double sum = 0.0;
@@ -264,11 +281,15 @@ int launch_distill(const dwarf_topk_distill_args& a, cudaStream_t stream) {
   const int bytes = (part * Vec16<T>::kVec + 31) / 32 * 4;
   if (a.grad == nullptr)
     return launch_rows(topk_distill_kernel<T, 128, false>, rows, cluster, 128, bytes, stream, a, cluster);
-  if (part <= 2048)
-    return launch_rows(topk_distill_kernel<T, 128, true>, rows, cluster, 128, bytes, stream, a, cluster);
-  if (part <= 4097)
-    return launch_rows(topk_distill_kernel<T, 256, true>, rows, cluster, 256, bytes, stream, a, cluster);
-  return launch_rows(topk_distill_kernel<T, 512, true>, rows, cluster, 512, bytes, stream, a, cluster);
+  const auto go = [&](auto kernel, auto again, int threads) {
+    // the same split of a row either way: the same bits
+    if (!a.skip_if_one || cluster > 1) return launch_rows(kernel, rows, cluster, threads, bytes, stream, a, cluster);
+    const int64_t wave = (int64_t)kNumSMs * (1024 / threads);
+    return launch_rows(again, rows < wave ? rows : wave, 1, threads, bytes, stream, a);
+  };
+  if (part <= 2048) return go(topk_distill_kernel<T, 128, true>, topk_distill_again_kernel<T, 128>, 128);
+  if (part <= 4097) return go(topk_distill_kernel<T, 256, true>, topk_distill_again_kernel<T, 256>, 256);
+  return go(topk_distill_kernel<T, 512, true>, topk_distill_again_kernel<T, 512>, 512);
 }
 
 }  // namespace

@@ -304,12 +304,11 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 9 : 8)
     // back into the sums. Otherwise d = c (x - m) and the bound is set in fp32.
     const typename V::Low low = V::low_of(m - 200.0f / c2);
     const float cm = m * c2;
-    if ((m - V::low_value(low)) * c2 >= 60.0f && fabsf(cm) < 1.0e30f && at + kVectors * kRowThreads <= part.size()) {
+    if ((m - V::low_value(low)) * c2 >= 60.0f && V::low_value(low) > -1.0e38f && fabsf(cm) < 1.0e30f) {
       const float2 shift = make_float2(-cm, -cm), cc = make_float2(c2, c2);
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i) {
+      auto add = [&](const uint4& w) {
         float2 e[V::kVec / 2];
-        V::unpack(V::clamp(v[i], low), e);
+        V::unpack(V::clamp(w, low), e);
 #pragma unroll
         for (int h = 0; h < V::kVec / 2; ++h) {
           const float2 d = fma2(e[h], cc, shift);
@@ -317,6 +316,14 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 9 : 8)
           s = add2(s, p);
           t = fma2(p, d, t);
         }
+      };
+      if (at + kVectors * kRowThreads <= part.size()) {
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) add(v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i)
+          if (at + i * kRowThreads < part.size()) add(v[i]);
       }
       const float left = fmaf(m, c2, -cm), f = ex2_approx(-left);
       const float s1 = s.x + s.y;

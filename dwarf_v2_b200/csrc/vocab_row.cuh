@@ -402,48 +402,59 @@ template <typename T, int kThreads = kRowThreads>
 struct Part {
   static constexpr int kVec = Vec16<T>::kVec;
   RowVectors<T> row;
-  int j0, j1;  // the part's vectors
+  int j0, j1;          // the part's vectors
+  int whole0, whole1;  // the row's whole vectors, up to the part's end
 
   __device__ __forceinline__ Part(const T* x, int vocab, int rank, int cluster) : row(x, vocab) {
     const int n = row.count(), per = ceil_div(n, cluster);
     j0 = min(rank * per, n);
     j1 = min(j0 + per, n);
+    whole0 = row.lead > 0 ? 1 : 0;
+    whole1 = min(j1, row.end / kVec);
   }
   __device__ __forceinline__ int size() const { return j1 - j0; }
-  // Whether all vectors of the tile that starts `at` vectors into the part are whole: its
-  // loops then need no checks (they cost a third of the instructions of the gradient).
+  // Whether all vectors of the tile that starts `at` vectors into the part, or of its step i, are
+  // whole: loops over them need no checks then (these cost a third of the instructions of
+  // the gradient).
   __device__ __forceinline__ bool full(int at) const {
-    return j0 + at >= (row.lead > 0 ? 1 : 0) && j0 + at + kVectors * kThreads <= min(j1, row.end / kVec);
+    return j0 + at >= whole0 && j0 + at + kVectors * kThreads <= whole1;
+  }
+  __device__ __forceinline__ bool full(int at, int i) const {
+    return j0 + at + i * kThreads >= whole0 && j0 + at + (i + 1) * kThreads <= whole1;
   }
   // Vectors at, at + threads, ...; places outside the part as -inf.
   __device__ __forceinline__ void load(int at, uint4 (&v)[kVectors]) const {
+    load_by(at, v, [](const uint4* p) { return ld_stream(p); });
+  }
+  __device__ __forceinline__ void load(int at, uint4 (&v)[kVectors], uint64_t policy) const {
+    load_by(at, v, [policy](const uint4* p) { return ld_stream(p, policy); });
+  }
+  template <typename F>
+  __device__ __forceinline__ void load_by(int at, uint4 (&v)[kVectors], F ld) const {
     const int j = j0 + at + threadIdx.x;
+    const uint4* p = reinterpret_cast<const uint4*>(row.base) + j;
     if (full(at)) {
-      const uint4* p = reinterpret_cast<const uint4*>(row.base) + j;
 #pragma unroll
-      for (int i = 0; i < kVectors; ++i) v[i] = ld_stream(p + i * kThreads);
+      for (int i = 0; i < kVectors; ++i) v[i] = ld(p + i * kThreads);
       return;
     }
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
-      v[i] = make_uint4(Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf);
-      if (j + i * kThreads < j1) v[i] = row.load(j + i * kThreads);
+      if (full(at, i)) {
+        v[i] = ld(p + i * kThreads);
+      } else {
+        v[i] = make_uint4(Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf);
+        if (j + i * kThreads < j1) v[i] = row.load(j + i * kThreads);
+      }
     }
-  }
-  // The same under an L2 policy.
-  __device__ __forceinline__ void load(int at, uint4 (&v)[kVectors], uint64_t policy) const {
-    if (!full(at)) return load(at, v);
-    const uint4* p = reinterpret_cast<const uint4*>(row.base) + (j0 + at + threadIdx.x);
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) v[i] = ld_stream(p + i * kThreads, policy);
   }
   // Asks L2 for the part's whole vectors under a policy, or for the first `most` of them; by one thread.
   __device__ __forceinline__ void prefetch_kept(uint64_t policy) const {
-    const int lo = max(j0, row.lead > 0 ? 1 : 0), hi = min(j1, row.end / kVec);
+    const int lo = max(j0, whole0), hi = whole1;
     if (lo < hi) prefetch_l2(reinterpret_cast<const uint4*>(row.base) + lo, (uint32_t)(hi - lo) * 16u, policy);
   }
   __device__ __forceinline__ void prefetch_first(int most) const {
-    const int lo = max(j0, row.lead > 0 ? 1 : 0), hi = min(min(j1, row.end / kVec), lo + most);
+    const int lo = max(j0, whole0), hi = min(whole1, lo + most);
     if (lo < hi) prefetch_l2(reinterpret_cast<const uint4*>(row.base) + lo, (uint32_t)(hi - lo) * 16u);
   }
   __device__ __forceinline__ bool holds(int id) const {
@@ -500,15 +511,20 @@ struct RowStore {
   template <int kThreads, typename F>
   __device__ __forceinline__ void tile(const Part<T, kThreads>& part, int at, const uint4 (&v)[kVectors], F f) const {
     const int j = part.j0 + at + threadIdx.x;
+    T* o = out + ((int64_t)j * kVec - row.lead);
     if (same && part.full(at)) {
-      T* o = out + ((int64_t)j * kVec - row.lead);
 #pragma unroll
       for (int i = 0; i < kVectors; ++i) st_stream(o + i * kThreads * kVec, f(v[i]));
       return;
     }
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i)
-      if (j + i * kThreads < part.j1) put(j + i * kThreads, f(v[i]));
+    for (int i = 0; i < kVectors; ++i) {
+      if (same && part.full(at, i)) {
+        st_stream(o + i * kThreads * kVec, f(v[i]));
+      } else if (j + i * kThreads < part.j1) {
+        put(j + i * kThreads, f(v[i]));
+      }
+    }
   }
   template <int kThreads>
   __device__ __forceinline__ void zero(const Part<T, kThreads>& part, int at) const {

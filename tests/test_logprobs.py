@@ -233,7 +233,7 @@ def test_top_order_of_hard_rows(R, V, dtype, kind):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
-@pytest.mark.parametrize("V", [50, 4096, 33001])
+@pytest.mark.parametrize("V", [50, 4096, 32768, 33001])
 def test_masked_and_special_rows(V, dtype):
     """-inf, the type's lowest value, +inf and NaN: in places, and in whole rows."""
     from dwarf_v2_b200.logprobs import token_logprobs
@@ -255,8 +255,8 @@ def test_masked_and_special_rows(V, dtype):
     x[11, :40] = -math.inf
     x[12] = torch.finfo(TYPES[dtype]).max
     x[13, 0] = torch.finfo(TYPES[dtype]).max
-    x = x.cuda()
-    targets = torch.full((14,), 1).cuda()
+    x = torch.cat([x, torch.where(torch.arange(V) % 5 == 0, low, -math.inf).to(x.dtype)[None]]).cuda()  # the lowest or nothing
+    targets = torch.full((15,), 1).cuda()
     targets[2], targets[4] = 0, 2
     for k in (1, 20, min(50, V)):
         check_forward(token_logprobs(x, targets, top_k=k), x, targets, k, 1.0)
