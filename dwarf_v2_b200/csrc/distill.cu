@@ -59,17 +59,18 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
     id = id64 < 0 ? -1 : id64 >= vocab ? vocab : (int)id64;
     if (id < 0) l = -CUDART_INF_F;
   }
-  const int words = (part.size() * V::kVec + 31) / 32;
+  const int words = ((part.j1 - part.j0) * V::kVec + 31) / 32;
   for (int i = tid; i < words; i += NT) listed[i] = 0;
   if (tid < k) s_id[tid] = id;
   if (tid == 0) s_flags = s_listed = 0;
   const RowStore<T> store(static_cast<T*>(a.grad) + r * a.vocab, part.row);
+  const int end_id = warp == 0 ? part.end_id(lane) : -1;
+  const float end = end_id >= 0 && counted ? to_f32(x[end_id]) : -CUDART_INF_F;
   const bool used = __syncthreads_or(id >= 0);
   if (cluster > 1) cluster_wait();
   if (!used) {  // the same for the whole cluster
     if (tid == 0 && rank == 0 && a.loss != nullptr) a.loss[r] = 0.0f;
-    if (kGrad)
-      for (int at = 0; at < part.size(); at += kTile) store.zero(part, at);
+    if (kGrad) store.zero(part);
     return;
   }
   const bool mine = id >= 0 && id < vocab && part.holds(id);
@@ -113,8 +114,9 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
     m = m_new;
     const float s = m == -CUDART_INF_F ? 0.0f : -m;
     // the bits of a thread's vectors of a tile lie NT kVec / 8 bytes apart
-    const unsigned char* bits = reinterpret_cast<const unsigned char*>(listed) + (at + tid) * V::kVec / 8;
-    const int bits_shift = V::kVec == 4 ? 4 * (tid & 1) : 0;
+    const int place = part.w0 - part.j0 + at + tid;
+    const unsigned char* bits = reinterpret_cast<const unsigned char*>(listed) + place * V::kVec / 8;
+    const int bits_shift = V::kVec == 4 ? 4 * (place & 1) : 0;
     auto add = [&](const uint4& w, uint32_t mask) {
       float2 e[V::kVec / 2];
       V::unpack(w, e);
@@ -145,6 +147,15 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
         add(v[i], in ? (bits[i * NT * V::kVec / 8] >> bits_shift) & ((1u << V::kVec) - 1u) : 0u);
       }
     }
+  }
+  if (warp == 0 && part.ends()) {
+    const float m_new = fmaxf(m, warp_max(end)), base = m_new == -CUDART_INF_F ? 0.0f : m_new;
+    const float f = ex2_approx((m - base) * c2), e = ex2_approx((end - base) * c2);
+    sum = mul2(sum, make_float2(f, f));
+    sum_list = mul2(sum_list, make_float2(f, f));
+    const int at = end_id + part.row.lead - part.j0 * V::kVec;
+    if (end_id >= 0 && ((listed[at >> 5] >> (at & 31)) & 1u)) sum_list.x += e; else sum.x += e;
+    m = m_new;
   }
   float s_r = warp_sum(sum.x + sum.y), s_l = warp_sum(sum_list.x + sum_list.y);
   if (lane == 0) s_m[warp] = m, s_rest[warp] = s_r, s_list[warp] = s_l;
@@ -220,6 +231,7 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
         return V::pack(e);
       });
     }
+    if (end_id >= 0) store.out[end_id] = from_f32<T>(ex2_approx((end - m) * c2) * k_rest);
   }
   __syncthreads();  // the listed entries are written again, with their own terms
   if (kGrad && mine) {
@@ -257,18 +269,30 @@ __global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_again_kernel(const
   }
 }
 
-__global__ void __launch_bounds__(1024) row_reduce_kernel(dwarf_row_reduce_args a) {
-  __shared__ double sd[32];
+// Sums in 64 bits, in an order that the launch fixes: the same bits every time.
+__global__ void __launch_bounds__(1024) row_reduce_kernel(const dwarf_row_reduce_args a) {
+  __shared__ double s_sum[32];
+  __shared__ int s_count[32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   double sum = 0.0;
-  for (int64_t i = threadIdx.x; i < a.rows; i += 1024) sum += a.values != nullptr ? (double)a.values[i] : (double)(a.mask[i] != 0);
-  sum = block_reduce<1024>(sum, sd, AddOp());
-  if (threadIdx.x != 0) return;
-  if (a.values == nullptr) {
-    *a.out = (float)(1.0 / fmax(1.0, sum));
-  } else {
-    const double scale = (a.scale != nullptr ? (double)*a.scale : 1.0) * (double)a.host_scale;
-    *a.out = (float)(sum * scale);
+  int count = 0;
+  for (int64_t i = tid; i < a.rows; i += blockDim.x) {
+    if (a.values != nullptr) sum += (double)a.values[i];
+    if (a.mask != nullptr) count += a.mask[i] != 0;
   }
+  sum = warp_sum(sum);
+  count = __reduce_add_sync(0xffffffffu, count);
+  if (lane == 0) s_sum[warp] = sum, s_count[warp] = count;
+  __syncthreads();
+  if (warp != 0) return;
+  const bool some = lane < (int)blockDim.x / 32;
+  sum = warp_sum(some ? s_sum[lane] : 0.0);
+  count = __reduce_add_sync(0xffffffffu, some ? s_count[lane] : 0);
+  if (lane != 0) return;
+  double out = a.values != nullptr ? sum * (double)a.host_scale : 1.0;
+  if (a.scale != nullptr) out *= (double)*a.scale;
+  if (a.mask != nullptr) out /= (double)max(count, 1);
+  *a.out = (float)out;
 }
 
 template <typename T>
@@ -318,8 +342,8 @@ extern "C" int dwarf_row_reduce(const dwarf_row_reduce_args* args, void* stream)
   using namespace dwarf;
   DWARF_CHECK_VERSION(args);
   const dwarf_row_reduce_args a = *args;
-  if (a.rows < 0) return DWARF_ERR_SHAPE;
+  if (a.rows < 0 || a.rows >= (1ll << 28)) return DWARF_ERR_SHAPE;
   if (a.out == nullptr || (a.rows > 0 && a.values == nullptr && a.mask == nullptr)) return DWARF_ERR_NULL;
-  row_reduce_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  row_reduce_kernel<<<1, a.rows <= 4096 ? 256 : 1024, 0, static_cast<cudaStream_t>(stream)>>>(a);
   return launch_status();
 }

@@ -111,7 +111,7 @@ __device__ __forceinline__ void bound_of_groups(const N* value, int groups, int 
 // part and its ties are taken in order.
 template <typename T>
 __device__ __forceinline__ int best_entries(const Part<T>& part, const typename Vec16<T>::Narrow* cells, int k,
-                                            bool nan, TopShared& sh) {
+                                            bool nan, float end, int end_id, TopShared& sh) {
   using N16 = Vec16<typename Vec16<T>::Narrow>;
   const int tid = threadIdx.x;
   uint32_t limit = sh.bound;
@@ -126,6 +126,7 @@ __device__ __forceinline__ int best_entries(const Part<T>& part, const typename 
         if (at < kHits) sh.hit[at] = c + N16::element(__ffs(m) - 1);
       }
     }
+    if (end_id >= 0 && end >= bound) sh.candidate[atomicAdd(&sh.n, 1)] = entry_key(end, (uint32_t)end_id);
     __syncthreads();
     const int hits = sh.hits;
     if (hits <= kHits) {
@@ -137,26 +138,18 @@ __device__ __forceinline__ int best_entries(const Part<T>& part, const typename 
 #pragma unroll
         for (int q = 0; q < kBatch; ++q) {  // the loads of a batch are in flight together
           const int h = first + q * kRowThreads + tid;
-          at_j[q] = part.j1;
+          at_j[q] = part.w1;
           if (h < items) {
             const int c = sh.hit[h / kCell];  // [tile][thread][cell]
-            at_j[q] = part.j0 + (c / (kCells * kRowThreads) * kVectors + h % kCell * kCells + c % kCells) * kRowThreads +
+            at_j[q] = part.w0 + (c / (kCells * kRowThreads) * kVectors + h % kCell * kCells + c % kCells) * kRowThreads +
                       c / kCells % kRowThreads;
           }
-          if (at_j[q] < part.j1) w[q] = part.row.load(at_j[q]);
+          if (at_j[q] < part.w1) w[q] = ld_stream(reinterpret_cast<const uint4*>(part.row.base) + at_j[q]);
         }
         uint32_t m[kBatch];
 #pragma unroll
         for (int q = 0; q < kBatch; ++q) {
-          m[q] = 0;
-          if (at_j[q] >= part.j1) continue;
-          m[q] = Vec16<T>::reach(w[q], bound);
-          if (m[q] != 0 && !part.row.whole(at_j[q])) {
-            for (uint32_t all = m[q]; all != 0; all &= all - 1) {
-              const int bit = __ffs(all) - 1, u = at_j[q] * Part<T>::kVec + Vec16<T>::element(bit);
-              if (u < part.row.lead || u >= part.row.end) m[q] &= ~(1u << bit);
-            }
-          }
+          m[q] = at_j[q] < part.w1 ? Vec16<T>::reach(w[q], bound) : 0u;
           found += __popc(m[q]);
         }
         if (found == 0) continue;
@@ -265,6 +258,8 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 9 : 8)
   if (cluster > 1) cluster_arrive();  // its CTAs have started, before one writes to another
 
   const Part<T> part(x, vocab, rank, cluster);
+  const int end_id = warp == 0 ? part.end_id(lane) : -1;
+  const float end = end_id >= 0 ? to_f32(x[end_id]) : -CUDART_INF_F;
   Sums sum = {-CUDART_INF_F, 0.0f, 0.0f};
   typename V::Max top0 = V::none(), top1 = V::none();  // maxima of the thread's even and odd vectors
   for (int at = 0; at < part.size(); at += kVectors * kRowThreads) {
@@ -349,6 +344,14 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 9 : 8)
     sum.s += s.x + s.y;
     sum.t += t.x + t.y;
   }
+  if (warp == 0 && part.ends()) {
+    const float m = fmaxf(sum.m, warp_max(end)), base = m == -CUDART_INF_F ? 0.0f : m;
+    const float d0 = fmaxf((sum.m - base) * c2, -200.0f), f = ex2_approx(d0);
+    const float d1 = (end - base) * c2, e = ex2_approx(d1);
+    sum.t = f * fmaf(d0, sum.s, sum.t) + e * fmaxf(d1, -200.0f);
+    sum.s = f * sum.s + e;
+    sum.m = m;
+  }
   // The next wave's row begins to arrive in L2 while this one's tail runs. In few waves the
   // tails leave memory idle (2047 rows of 32768 bf16, 5 alternatives: 37.0 us without, 34.9
   // with; 4096 of fp32: 94.6, 86.5); in many the CTAs have drifted apart, and only rows
@@ -395,7 +398,7 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 9 : 8)
     bool nan = false;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) nan |= s_warp[w].s != s_warp[w].s;
-    n = best_entries(part, s_cells, k, nan, top);
+    n = best_entries(part, s_cells, k, nan, end, end_id, top);
   }
   if (cluster > 1) {
     if (kTop) {
@@ -522,7 +525,7 @@ __global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
   const float g_h = a.g_entropy != nullptr ? a.g_entropy[r] : 0.0f;
   any = __syncthreads_or(any) || g_lse != 0.0f || g_h != 0.0f;
   if (!any || ms.y == 0.0f) {
-    for (int at = 0; at < part.size(); at += kVectors * kRowThreads) store.zero(part, at);
+    store.zero(part);
     return;
   }
   const float weight = off ? CUDART_NAN_F : g - g_lse;
@@ -547,6 +550,11 @@ __global__ void __launch_bounds__(kRowThreads, 1024 / kRowThreads)
       for (int h = 0; h < V::kVec / 2; ++h) e[h] = dense(e[h]);
       return V::pack(e);
     });
+  }
+  const int end_id = tid < 32 ? part.end_id(tid) : -1;
+  if (end_id >= 0) {
+    const float v = to_f32(x[end_id]);
+    store.out[end_id] = from_f32<T>(dense(make_float2(v, v)).x);
   }
   __syncthreads();  // the listed entries are written again, with their own terms
   for (int j = tid; j < n; j += kRowThreads) {

@@ -327,12 +327,15 @@ struct RowVectors {
   __device__ __forceinline__ bool whole(int j) const { return j * kVec >= lead && (j + 1) * kVec <= end; }
   __device__ __forceinline__ uint4 load(int j) const {
     if (whole(j)) return ld_stream(base + (int64_t)j * kVec);
-    uint4 v = make_uint4(Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf);
+    // the nearest element of the row for a place outside it, so that no load waits for a branch
+    uint4 v;
     T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) e[i] = base[min(max(j * kVec + i, lead), end - 1)];
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       const int u = j * kVec + i;
-      if (u >= lead && u < end) e[i] = base[u];
+      if (u < lead || u >= end) e[i] = from_f32<T>(-CUDART_INF_F);
     }
     return v;
   }
@@ -397,32 +400,29 @@ int launch_rows(void (*kernel)(Params...), int64_t rows, int cluster, int thread
   return launch_status();
 }
 
-// A CTA's part of a row, a tile of kVectors vectors for each thread at a time.
+// A CTA's part of a row: its whole vectors, a tile of kVectors vectors for each thread at
+// a time, and the up to 2 (kVec - 1) elements at the row's ends that fill no vector, one for each of
+// a warp's first 16 lanes. (Ends inside the tiles' loops made the odd vocabulary of 32003 take
+// 228 us where 32768 took 155: 6000 rows, distillation with gradient.)
 template <typename T, int kThreads = kRowThreads>
 struct Part {
   static constexpr int kVec = Vec16<T>::kVec;
   RowVectors<T> row;
-  int j0, j1;          // the part's vectors
-  int whole0, whole1;  // the row's whole vectors, up to the part's end
+  int j0, j1;  // the part's vectors
+  int w0, w1;  // those of them that are whole
 
   __device__ __forceinline__ Part(const T* x, int vocab, int rank, int cluster) : row(x, vocab) {
     const int n = row.count(), per = ceil_div(n, cluster);
     j0 = min(rank * per, n);
     j1 = min(j0 + per, n);
-    whole0 = row.lead > 0 ? 1 : 0;
-    whole1 = min(j1, row.end / kVec);
+    w0 = max(j0, row.lead > 0 ? 1 : 0);
+    w1 = max(w0, min(j1, row.end / kVec));
   }
-  __device__ __forceinline__ int size() const { return j1 - j0; }
-  // Whether all vectors of the tile that starts `at` vectors into the part, or of its step i, are
-  // whole: loops over them need no checks then (these cost a third of the instructions of
-  // the gradient).
-  __device__ __forceinline__ bool full(int at) const {
-    return j0 + at >= whole0 && j0 + at + kVectors * kThreads <= whole1;
-  }
-  __device__ __forceinline__ bool full(int at, int i) const {
-    return j0 + at + i * kThreads >= whole0 && j0 + at + (i + 1) * kThreads <= whole1;
-  }
-  // Vectors at, at + threads, ...; places outside the part as -inf.
+  __device__ __forceinline__ int size() const { return w1 - w0; }
+  // Whether the tile that starts `at` vectors into the part, or its step i, has a vector for every thread.
+  __device__ __forceinline__ bool full(int at) const { return at + kVectors * kThreads <= size(); }
+  __device__ __forceinline__ bool full(int at, int i) const { return at + (i + 1) * kThreads <= size(); }
+  // Vectors at, at + threads, ...; past the part -inf.
   __device__ __forceinline__ void load(int at, uint4 (&v)[kVectors]) const {
     load_by(at, v, [](const uint4* p) { return ld_stream(p); });
   }
@@ -431,8 +431,7 @@ struct Part {
   }
   template <typename F>
   __device__ __forceinline__ void load_by(int at, uint4 (&v)[kVectors], F ld) const {
-    const int j = j0 + at + threadIdx.x;
-    const uint4* p = reinterpret_cast<const uint4*>(row.base) + j;
+    const uint4* p = reinterpret_cast<const uint4*>(row.base) + (w0 + at + (int)threadIdx.x);
     if (full(at)) {
 #pragma unroll
       for (int i = 0; i < kVectors; ++i) v[i] = ld(p + i * kThreads);
@@ -440,22 +439,24 @@ struct Part {
     }
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
-      if (full(at, i)) {
-        v[i] = ld(p + i * kThreads);
-      } else {
-        v[i] = make_uint4(Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf);
-        if (j + i * kThreads < j1) v[i] = row.load(j + i * kThreads);
-      }
+      v[i] = make_uint4(Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf, Vec16<T>::kMinusInf);
+      if (at + i * kThreads + (int)threadIdx.x < size()) v[i] = ld(p + i * kThreads);
     }
+  }
+  // Whether the row has ends; the id of the element of them that a lane has, or -1.
+  __device__ __forceinline__ bool ends() const { return row.lead > 0 || row.end % kVec > 0; }
+  __device__ __forceinline__ int end_id(int lane) const {
+    const int tail = max(row.end / kVec, row.lead > 0 ? 1 : 0);
+    const int j = lane < 8 ? 0 : tail, u = lane < 8 ? row.lead + lane : tail * kVec + lane - 8;
+    const int last = lane < 8 ? (row.lead > 0 ? min(kVec, row.end) : 0) : lane < 16 ? row.end : 0;
+    return u < last && j >= j0 && j < j1 ? u - row.lead : -1;
   }
   // Asks L2 for the part's whole vectors under a policy, or for the first `most` of them; by one thread.
   __device__ __forceinline__ void prefetch_kept(uint64_t policy) const {
-    const int lo = max(j0, whole0), hi = whole1;
-    if (lo < hi) prefetch_l2(reinterpret_cast<const uint4*>(row.base) + lo, (uint32_t)(hi - lo) * 16u, policy);
+    if (size() > 0) prefetch_l2(reinterpret_cast<const uint4*>(row.base) + w0, (uint32_t)size() * 16u, policy);
   }
   __device__ __forceinline__ void prefetch_first(int most) const {
-    const int lo = max(j0, whole0), hi = min(whole1, lo + most);
-    if (lo < hi) prefetch_l2(reinterpret_cast<const uint4*>(row.base) + lo, (uint32_t)(hi - lo) * 16u);
+    if (size() > 0) prefetch_l2(reinterpret_cast<const uint4*>(row.base) + w0, (uint32_t)min(size(), most) * 16u);
   }
   __device__ __forceinline__ bool holds(int id) const {
     const int j = (id + row.lead) / kVec;
@@ -490,28 +491,15 @@ template <typename T>
 struct RowStore {
   static constexpr int kVec = Vec16<T>::kVec;
   T* out;
-  const RowVectors<T>& row;
+  int lead;
   bool same;
-  __device__ __forceinline__ RowStore(T* o, const RowVectors<T>& r) : out(o), row(r) {
+  __device__ __forceinline__ RowStore(T* o, const RowVectors<T>& r) : out(o), lead(r.lead) {
     same = (reinterpret_cast<uintptr_t>(o) & 15) == r.lead * sizeof(T);
-  }
-  __device__ __forceinline__ void put(int j, const uint4& v) const {
-    if (same && row.whole(j)) {
-      st_stream(out + ((int64_t)j * kVec - row.lead), v);
-      return;
-    }
-    const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const int u = j * kVec + i;
-      if (u >= row.lead && u < row.end) out[u - row.lead] = e[i];
-    }
   }
   // f of each vector of a tile of `part`, stored.
   template <int kThreads, typename F>
   __device__ __forceinline__ void tile(const Part<T, kThreads>& part, int at, const uint4 (&v)[kVectors], F f) const {
-    const int j = part.j0 + at + threadIdx.x;
-    T* o = out + ((int64_t)j * kVec - row.lead);
+    T* o = out + ((int64_t)(part.w0 + at + (int)threadIdx.x) * kVec - lead);
     if (same && part.full(at)) {
 #pragma unroll
       for (int i = 0; i < kVectors; ++i) st_stream(o + i * kThreads * kVec, f(v[i]));
@@ -519,17 +507,24 @@ struct RowStore {
     }
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
-      if (same && part.full(at, i)) {
-        st_stream(o + i * kThreads * kVec, f(v[i]));
-      } else if (j + i * kThreads < part.j1) {
-        put(j + i * kThreads, f(v[i]));
+      if (at + i * kThreads + (int)threadIdx.x >= part.size()) break;
+      const uint4 w = f(v[i]);
+      if (same) {
+        st_stream(o + i * kThreads * kVec, w);
+      } else {
+        const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+        for (int h = 0; h < kVec; ++h) o[i * kThreads * kVec + h] = e[h];
       }
     }
   }
+  // Zeros in the part.
   template <int kThreads>
-  __device__ __forceinline__ void zero(const Part<T, kThreads>& part, int at) const {
+  __device__ __forceinline__ void zero(const Part<T, kThreads>& part) const {
     const uint4 v[kVectors] = {};
-    tile(part, at, v, [](const uint4& w) { return w; });
+    for (int at = 0; at < part.size(); at += kVectors * kThreads) tile(part, at, v, [](const uint4& w) { return w; });
+    const int id = threadIdx.x < 32 ? part.end_id(threadIdx.x) : -1;
+    if (id >= 0) out[id] = from_f32<T>(0.0f);
   }
 };
 

@@ -40,10 +40,10 @@ def _launch(logits, ids, logprobs, mask, inv_temperature, tail, *, loss=None, gr
         _rows.launch("dwarf_topk_distill", args, logits.device)
 
 
-def _reduce(out, *, values=None, mask=None, scale=None, host_scale=1.0) -> None:
+def _reduce(out, *, values=None, mask=None, host_scale=1.0) -> None:
     rows = (values if values is not None else mask).numel()
     args = _lib.RowReduceArgs(version=_lib.ABI_VERSION, rows=rows, values=_lib.ptr(values), mask=_lib.ptr(mask),
-                              scale=_lib.ptr(scale), host_scale=host_scale, out=out.data_ptr())
+                              host_scale=host_scale, out=out.data_ptr())
     _rows.launch("dwarf_row_reduce", args, out.device)
 
 
@@ -61,8 +61,9 @@ class _TopKDistillationFn(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        if torch.is_grad_enabled():  # create_graph: a second derivative is refused, not left out
+            return _once_more(ctx, g)
         logits, ids, logprobs, mask = ctx.saved_tensors
         grad, ctx.grad = ctx.grad, None  # a second backward gets a buffer of its own
         written = grad is not None
@@ -71,6 +72,9 @@ class _TopKDistillationFn(torch.autograd.Function):
         _launch(logits, ids, logprobs, mask, *ctx.scalars, grad=grad, grad_scale=ctx.grad_scale,
                 grad_rows=g.contiguous(), skip_if_one=written, scale=ctx.scale)
         return grad, None, None, None, None, None, None, None
+
+
+_once_more = torch.autograd.function.once_differentiable(_TopKDistillationFn.backward)
 
 
 def _forward(logits, ids, logprobs, mask, inv_temperature, tail, reduction, weight, grad):
@@ -83,7 +87,7 @@ def _forward(logits, ids, logprobs, mask, inv_temperature, tail, reduction, weig
     if reduction == "mean":
         if mask is None:
             scale = weight / rows.numel()
-        else:
+        elif grad is not None:  # the gradient needs the number of rows before the loss is there
             grad_scale = torch.empty((), dtype=torch.float32, device=dev)
             _reduce(grad_scale, mask=mask)
     _launch(logits, ids, logprobs, mask, inv_temperature, tail, loss=rows, grad=grad, grad_scale=grad_scale,
@@ -91,8 +95,12 @@ def _forward(logits, ids, logprobs, mask, inv_temperature, tail, reduction, weig
     if reduction == "none":
         return rows, scale, grad_scale
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    host = 1.0 / rows.numel() if reduction == "mean" and mask is None else 1.0
-    _reduce(loss, values=rows, scale=grad_scale, host_scale=host)
+    if reduction == "sum":
+        _reduce(loss, values=rows)
+    elif mask is None:
+        _reduce(loss, values=rows, host_scale=1.0 / rows.numel())
+    else:
+        _reduce(loss, values=rows, mask=mask)
     return loss, scale, grad_scale
 
 

@@ -69,8 +69,9 @@ class _TokenLogprobsFn(torch.autograd.Function):
         return logprob, entropy, lse, top_logprobs, top_ids
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_logprob, g_entropy, g_lse, g_top, _):
+    def backward(ctx, g_logprob, g_entropy, g_lse, g_top, no_grad):
+        if torch.is_grad_enabled():  # create_graph: a second derivative is refused, not left out
+            return _once_more(ctx, g_logprob, g_entropy, g_lse, g_top, no_grad)
         logits, targets, entropy, stats, top_ids = ctx.saved_tensors
         top_k, inv_temperature, ignore_index = ctx.scalars
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
@@ -86,6 +87,9 @@ class _TokenLogprobsFn(torch.autograd.Function):
         if outer * inner:
             _rows.launch("dwarf_token_logprobs_bwd", args, logits.device)
         return grad, None, None, None, None
+
+
+_once_more = torch.autograd.function.once_differentiable(_TokenLogprobsFn.backward)
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *, top_k: int = 0,

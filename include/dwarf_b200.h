@@ -839,16 +839,16 @@ typedef struct {
 
 int dwarf_topk_distill(const dwarf_topk_distill_args* args, void* stream);
 
-/* One fp32 value from rows: with `values`, out = (scale ? *scale : 1) * sum of
- * values in a fixed order; without, out = 1 / max(1, number of mask bytes set),
- * the scale of a mean over the rows that count. */
+/* One fp32 value from rows, summed in 64 bits in a fixed order:
+ *   out = [values: host_scale * sum of values; else 1] * [scale: *scale] / [mask: max(1, mask bytes set)]
+ * the reduced loss, or (without values) the scale of a mean over the rows that count. */
 typedef struct {
   int32_t version;
   int64_t rows;
   const float* values;            /* optional [rows]                       */
-  const uint8_t* mask;            /* [rows] (without values)               */
+  const uint8_t* mask;            /* optional [rows]                       */
   const float* scale;             /* optional device scalar                */
-  float host_scale;               /* a further factor                      */
+  float host_scale;
   float* out;                     /* [1]                                   */
 } dwarf_row_reduce_args;
 

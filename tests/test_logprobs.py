@@ -379,6 +379,22 @@ def test_strides_and_alignment(dtype):
 
 
 @pytest.mark.gpu
+def test_second_derivative_is_refused():
+    from dwarf_v2_b200.distillation import topk_distillation_loss
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    x = logits(3, 64, "fp32", 0).cuda().requires_grad_()
+    ids = torch.arange(4).repeat(3, 1).cuda()
+    lp = torch.full((3, 4), -2.0).cuda()
+    for value in (token_logprobs(x, torch.tensor([1, 2, 3]).cuda()).logprob.sum(), topk_distillation_loss(x, ids, lp)):
+        plain, = torch.autograd.grad(value, x, retain_graph=True)
+        grad, = torch.autograd.grad(value, x, create_graph=True)
+        assert torch.equal(grad.detach(), plain)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(grad.sum(), x)
+
+
+@pytest.mark.gpu
 def test_no_rows_and_neighbours_untouched():
     from dwarf_v2_b200 import _lib, _rows
     from dwarf_v2_b200.logprobs import token_logprobs
