@@ -8,6 +8,10 @@ Drop-in modules mirroring the reference's public API:
                                                (kernels/hierarchical_sparse_attn_v18_hisa.py)
 * ``dwarf_v2_b200.model``                      (model construction of train/train_dwarf.py)
 
+Beyond the reference: ``dwarf_v2_b200.logprobs`` (log probabilities of given tokens with
+entropy and top alternatives, differentiable) and ``dwarf_v2_b200.distillation`` (the loss
+against a teacher's top log probabilities, forward and backward).
+
 All device work runs in hand-written sm_100a CUDA kernels behind the C ABI
 declared in include/dwarf_b200.h (``libdwarf_b200.so``): the attention, scan and
 glue kernels and a tcgen05 GEMM with fused epilogues. A few projection GEMMs of

@@ -441,6 +441,55 @@ def case_model_train_step(timer, peak):
             "kernels_mean_ms": timer(step, names)}
 
 
+def _vocab_rows(rows: int, vocab: int = 32768):
+    """Logit rows with a token-frequency bias: what the model's lm_head gives a trained model."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    bias = -1.2 * torch.log(torch.randperm(vocab, generator=g, device="cuda") + 3.0) + 6.0
+    return (torch.randn(rows, vocab, generator=g, device="cuda") * 1.6 + bias).to(torch.bfloat16), g
+
+
+def case_logprobs_rows16k(timer, peak):
+    """Token log probabilities of 8 x 2048 rows of the model's vocabulary (bf16): scoring without
+    alternatives, a teacher's pass with 64, and the gradient of log probability + entropy."""
+    from .logprobs import token_logprobs
+
+    x, g = _vocab_rows(8 * 2048)
+    targets = torch.randint(0, x.shape[1], (x.shape[0],), generator=g, device="cuda")
+    name, back = "dwarf_token_logprobs", "dwarf_token_logprobs_bwd"
+    score = timer(lambda: token_logprobs(x, targets), (name,))[name]
+    teacher = timer(lambda: token_logprobs(x, targets, top_k=64, temperature=2.0), (name,))[name]
+    leaf = x.requires_grad_()
+    w = torch.full((x.shape[0],), 1.0 / x.shape[0], device="cuda")
+
+    def step():
+        out = token_logprobs(leaf, targets)
+        torch.autograd.grad([out.logprob, out.entropy], leaf, [w, w])
+
+    grad = timer(step, (back,))[back]
+    return {"score": _rate(_nbytes(x), score, peak), "top_k_64": _rate(_nbytes(x), teacher, peak),
+            "gradient": _rate(2 * _nbytes(x), grad, peak)}
+
+
+def case_distill_rows16k(timer, peak):
+    """Distillation from a teacher's 64 top entries on 8 x 2048 rows of the model's vocabulary
+    (bf16): the loss alone, and the loss with the gradient of the logits from one launch."""
+    from .distillation import topk_distillation_loss
+    from .logprobs import token_logprobs
+
+    x, g = _vocab_rows(8 * 2048)
+    with torch.no_grad():
+        top = token_logprobs(x.roll(1, 0), top_k=64, temperature=2.0)
+    name = "dwarf_topk_distill"
+
+    def loss(logits):
+        return topk_distillation_loss(logits, top.top_ids, top.top_logprobs, temperature=2.0)
+
+    alone = timer(lambda: loss(x), (name,))[name]
+    leaf = x.requires_grad_()
+    grad = timer(lambda: loss(leaf), (name,))[name]
+    return {"loss": _rate(_nbytes(x), alone, peak), "loss_and_gradient": _rate(2 * _nbytes(x), grad, peak)}
+
+
 CASES = {
     "ema_config2": case_ema_config2,
     "ema_model_bf16": case_ema_model_bf16,
@@ -457,6 +506,8 @@ CASES = {
     "dsqg_bwd_model_group": case_dsqg_bwd_model_group,
     "hisa_config4": case_hisa_config4,
     "hisa_bwd_config4": case_hisa_bwd_config4,
+    "logprobs_rows16k": case_logprobs_rows16k,
+    "distill_rows16k": case_distill_rows16k,
     "model_train_step": case_model_train_step,
 }
 

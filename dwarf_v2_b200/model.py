@@ -19,7 +19,8 @@ the reference's rounding points.
 Calls that need gradients (training mode, or autograd on with parameters that
 require grad) take the reference's own block formulas as torch ops over the
 engine's differentiable DSQG, HISA and EMA-scan functions (forward and backward
-kernels); ``forward_lse`` and the decode entry points are inference-only.
+kernels); ``forward_lse``, ``forward_logprobs`` and the decode entry points are
+inference-only.
 """
 
 from __future__ import annotations
@@ -36,6 +37,7 @@ from . import _lib, gemm, glue
 from .causal_ema_scan import bounded_ema_factor, causal_ema_scan, inverse_bounded_ema_factor
 from .dsqg_attention_v22 import ALL_OFFSETS, R_PLANES, DSQGAttentionV19
 from .hierarchical_sparse_attn_v18_hisa import HierarchicalSparseAttentionV16HISACausal, chunk_representatives
+from .logprobs import TokenLogprobs, token_logprobs
 
 EXPECTED_PARAMETERS = 55_348_728
 EXPECTED_TRAINABLE_PARAMETERS = 55_344_120
@@ -561,6 +563,29 @@ class DwarfForCausalLM(nn.Module):
                                             None if labels is None else labels.reshape(-1))
         shape = (B, T)
         return lse.view(shape), argmax.view(shape), None if loss is None else loss.view(shape)
+
+    def forward_logprobs(self, input_ids: torch.Tensor, targets: torch.Tensor | None = None, *, top_k: int = 0,
+                         temperature: float = 1.0, ignore_index: int = -100) -> TokenLogprobs:
+        """Per-token log probability of ``targets`` [B, T] (or None), entropy, lse and the ``top_k``
+        best alternatives at ``temperature`` (see ``logprobs.token_logprobs``), from bf16 logits as
+        ``forward`` computes them. The logits are made 1024 rows at a time, so that [B, T, vocab] never
+        exists and each piece is read back from L2. Inference only; its ``top_ids`` and
+        ``top_logprobs`` are what ``distillation.topk_distillation_loss`` takes from a teacher."""
+        self._check(input_ids, inference_only=True)
+        B, T = input_ids.shape
+        if targets is not None and tuple(targets.shape) != (B, T):
+            raise ValueError(f"targets must be {(B, T)}, got {tuple(targets.shape)}")
+        hidden = self.forward_hidden(input_ids).reshape(B * T, -1)
+        weight = _act(self.embedding.weight.detach()).contiguous()
+        flat = None if targets is None else targets.reshape(-1)
+        parts = []
+        for at in range(0, max(1, B * T), 1024):
+            rows = slice(at, min(at + 1024, B * T))
+            logits = gemm.linear(hidden[rows], weight) if B * T else hidden.new_empty(0, weight.shape[0])
+            parts.append(token_logprobs(logits, None if flat is None else flat[rows], top_k=top_k,
+                                        temperature=temperature, ignore_index=ignore_index))
+        fields = [None if f[0] is None else torch.cat(f).reshape(B, T, *f[0].shape[1:]) for f in zip(*parts)]
+        return TokenLogprobs(*fields)
 
     # ------------------------------------------------------------------ incremental decoding
 
