@@ -30,8 +30,9 @@ __device__ __forceinline__ void warp_join(float c2, float& m, float& a, float& b
 template <typename T, int NT, bool kGrad>
 __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, int cluster, int64_t r) {
   using V = Vec16<T>;
-  constexpr int kWarps = NT / 32, kTile = kVectors * NT, kListWarps = DWARF_TOP_K_MAX / 32;
-  static_assert(NT >= DWARF_TOP_K_MAX, "one thread for each slot of the teacher's list");
+  constexpr int kWarps = NT / 32, kTile = kVectors * NT;
+  constexpr int kSlots = NT < DWARF_TOP_K_MAX ? DWARF_TOP_K_MAX / NT : 1;  // slots of the teacher's list for a thread
+  constexpr int kListWarps = NT < DWARF_TOP_K_MAX ? kWarps : DWARF_TOP_K_MAX / 32;
   extern __shared__ __align__(16) uint32_t listed[];  // a bit for each place of the part
   __shared__ float s_m[kWarps], s_rest[kWarps], s_list[kWarps];
   __shared__ float s_top[kListWarps], s_term[kListWarps];
@@ -48,48 +49,70 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
   const Part<T, NT> part(x, vocab, rank, cluster);
   const uint64_t keep = kGrad ? policy_keep() : 0;
 
-  // the teacher's slots, one a thread
+  // the teacher's slots
   const bool counted = a.row_mask == nullptr || a.row_mask[r] != 0;
   if (kGrad && tid == 0 && counted) part.prefetch_kept(keep);
-  int id = -1;  // not used; vocab: past the vocabulary
-  float l = -CUDART_INF_F;
-  if (tid < k && counted) {
-    const int64_t id64 = a.teacher_ids[r * k + tid];
-    l = a.teacher_logprobs[r * k + tid];
-    id = id64 < 0 ? -1 : id64 >= vocab ? vocab : (int)id64;
-    if (id < 0) l = -CUDART_INF_F;
+  int id[kSlots];  // -1: not used; vocab: past the vocabulary
+  float l[kSlots];
+#pragma unroll
+  for (int s = 0; s < kSlots; ++s) {
+    const int slot = tid + s * NT;
+    id[s] = -1;
+    l[s] = -CUDART_INF_F;
+    if (slot < k && counted) {
+      const int64_t id64 = a.teacher_ids[r * k + slot];
+      l[s] = a.teacher_logprobs[r * k + slot];
+      id[s] = id64 < 0 ? -1 : id64 >= vocab ? vocab : (int)id64;
+      if (id[s] < 0) l[s] = -CUDART_INF_F;
+    }
   }
   const int words = ((part.j1 - part.j0) * V::kVec + 31) / 32;
   for (int i = tid; i < words; i += NT) listed[i] = 0;
-  if (tid < k) s_id[tid] = id;
+  bool any = false;
+#pragma unroll
+  for (int s = 0; s < kSlots; ++s) {
+    if (tid + s * NT < k) s_id[tid + s * NT] = id[s];
+    any |= id[s] >= 0;
+  }
   if (tid == 0) s_flags = s_listed = 0;
   const RowStore<T> store(static_cast<T*>(a.grad) + r * a.vocab, part.row);
   const int end_id = warp == 0 ? part.end_id(lane) : -1;
   const float end = end_id >= 0 && counted ? to_f32(x[end_id]) : -CUDART_INF_F;
-  const bool used = __syncthreads_or(id >= 0);
+  const bool used = __syncthreads_or(any);
   if (cluster > 1) cluster_wait();
   if (!used) {  // the same for the whole cluster
     if (tid == 0 && rank == 0 && a.loss != nullptr) a.loss[r] = 0.0f;
     if (kGrad) store.zero(part);
     return;
   }
-  const bool mine = id >= 0 && id < vocab && part.holds(id);
-  if (mine) {
-    const int at = id + part.row.lead - part.j0 * V::kVec;
-    const uint32_t bit = 1u << (at & 31);
-    if (atomicOr(&listed[at >> 5], bit) & bit) atomicOr(&s_flags, 1);  // an id that another slot has too
+  float xv[kSlots];
+#pragma unroll
+  for (int s = 0; s < kSlots; ++s) {
+    if (id[s] >= 0 && id[s] < vocab && part.holds(id[s])) {
+      const int at = id[s] + part.row.lead - part.j0 * V::kVec;
+      const uint32_t bit = 1u << (at & 31);
+      if (atomicOr(&listed[at >> 5], bit) & bit) atomicOr(&s_flags, 1);  // an id that another slot has too
+    }
+    if (id[s] >= vocab) atomicOr(&s_flags, 2);
+    xv[s] = to_f32(x[id[s] >= 0 && id[s] < vocab ? id[s] : 0]);
   }
-  if (id >= vocab) atomicOr(&s_flags, 2);
-  const float xv = to_f32(x[id >= 0 && id < vocab ? id : 0]);
   // sum p for a teacher with a tail, in 64 bits (the rest, 1 - sum p, may be far below 1); else the
   // list's maximum and the sum relative to it
   if (warp < kListWarps) {
     if (a.tail) {
-      const double sum = warp_sum(id >= 0 ? exp((double)l) : 0.0);
+      double sum = 0.0;
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s) sum += id[s] >= 0 ? exp((double)l[s]) : 0.0;
+      sum = warp_sum(sum);
       if (lane == 0) s_sum[warp] = sum;
     } else {
-      const float top = warp_max(l);
-      const float sum = warp_sum(l > -CUDART_INF_F ? expf(l - top) : l == l ? 0.0f : l);
+      float top = l[0], sum = 0.0f;
+#pragma unroll
+      for (int s = 1; s < kSlots; ++s) top = fmaxf(top, l[s]);
+      top = warp_max(top);
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s) sum += l[s] > -CUDART_INF_F ? expf(l[s] - top) : l[s] == l[s] ? 0.0f : l[s];
+      sum = warp_sum(sum);
       if (lane == 0) s_top[warp] = top, s_sum[warp] = sum;
     }
   }
@@ -198,16 +221,24 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
 #pragma unroll
     for (int w = 0; w < kListWarps; ++w)
       sum_p += s_sum[w] == 0.0 ? 0.0f : (float)s_sum[w] * expf(s_top[w] - top);
-    l = l - top - logf(sum_p);
+    const float ln_sum = logf(sum_p);
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) l[s] = l[s] - top - ln_sum;
     if (!(sum_p > 0.0f)) weight = CUDART_NAN_F;  // no slot with a finite value
   }
   if (off) weight = CUDART_NAN_F;
-  const float p = id >= 0 ? expf(l) : 0.0f;
+  float p[kSlots], term = 0.0f;
+  const float ln_total = log2f(total) * kLn2;
+#pragma unroll
+  for (int s = 0; s < kSlots; ++s) {
+    p[s] = id[s] >= 0 ? expf(l[s]) : 0.0f;
+    term += p[s] > 0.0f ? p[s] * (l[s] - (xv[s] - m) * a.inv_temperature + ln_total) : p[s];
+    if (tid + s * NT < k) s_p[tid + s * NT] = p[s];
+  }
   if (a.loss != nullptr && warp < kListWarps) {
-    const float term = warp_sum(p > 0.0f ? p * (l - (xv - m) * a.inv_temperature + log2f(total) * kLn2) : p);
+    term = warp_sum(term);
     if (lane == 0) s_term[warp] = term;
   }
-  if (tid < k) s_p[tid] = p;
   float sc = 0.0f, k_list = 0.0f;
   if (kGrad) {
     sc = a.scale * a.inv_temperature;
@@ -234,20 +265,24 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
     if (end_id >= 0) store.out[end_id] = from_f32<T>(ex2_approx((end - m) * c2) * k_rest);
   }
   __syncthreads();  // the listed entries are written again, with their own terms
-  if (kGrad && mine) {
-    float taken = p;
-    if (s_flags & 1) {
-      taken = 0.0f;
-      for (int j = 0; j < k; ++j)
-        if (s_id[j] == id) taken += s_p[j];
+  if (kGrad) {
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      if (id[s] < 0 || id[s] >= vocab || !part.holds(id[s])) continue;
+      float taken = p[s];
+      if (s_flags & 1) {
+        taken = 0.0f;
+        for (int j = 0; j < k; ++j)
+          if (s_id[j] == id[s]) taken += s_p[j];
+      }
+      store.out[id[s]] = from_f32<T>(ex2_approx((xv[s] - m) * c2) * k_list - sc * taken);
     }
-    store.out[id] = from_f32<T>(ex2_approx((xv - m) * c2) * k_list - sc * taken);
   }
   if (a.loss != nullptr && rank == 0 && tid == 0) {
-    float term = 0.0f;
+    term = 0.0f;
 #pragma unroll
     for (int w = 0; w < kListWarps; ++w) term += s_term[w];
-    if (!(rest <= 0.0f)) term += rest * (logf(rest) - (log2f(s_r) - log2f(total)) * kLn2);
+    if (!(rest <= 0.0f)) term += rest * (logf(rest) - log2f(s_r) * kLn2 + ln_total);
     a.loss[r] = off ? CUDART_NAN_F : term * a.loss_scale;
   }
 }
@@ -303,6 +338,8 @@ int launch_distill(const dwarf_topk_distill_args& a, cudaStream_t stream) {
   // a row that starts off a 16-byte boundary has one vector more
   const int part = ceil_div(vectors + 1, cluster);
   const int bytes = (part * Vec16<T>::kVec + 31) / 32 * 4;
+  if (a.grad == nullptr && warp_rows(rows, vectors, 2048))
+    return launch_rows(topk_distill_kernel<T, 32, false>, rows, 1, 32, bytes, stream, a, 1);
   if (a.grad == nullptr)
     return launch_rows(topk_distill_kernel<T, 128, false>, rows, cluster, 128, bytes, stream, a, cluster);
   const auto go = [&](auto kernel, auto again, int threads) {
@@ -311,6 +348,8 @@ int launch_distill(const dwarf_topk_distill_args& a, cudaStream_t stream) {
     const int64_t wave = (int64_t)kNumSMs * (1024 / threads);
     return launch_rows(again, rows < wave ? rows : wave, 1, threads, bytes, stream, a);
   };
+  // 32768 rows of 4096 bf16: 226 us with 128 threads, 137 with a warp; 16384 of 4096 fp32: 111, 129
+  if (warp_rows(rows, vectors, 512)) return go(topk_distill_kernel<T, 32, true>, topk_distill_again_kernel<T, 32>, 32);
   if (part <= 2048) return go(topk_distill_kernel<T, 128, true>, topk_distill_again_kernel<T, 128>, 128);
   if (part <= 4097) return go(topk_distill_kernel<T, 256, true>, topk_distill_again_kernel<T, 256>, 256);
   return go(topk_distill_kernel<T, 512, true>, topk_distill_again_kernel<T, 512>, 512);

@@ -170,7 +170,7 @@ def test_c_entry_refuses_bad_arguments():
 @pytest.mark.parametrize("tail", [True, False])
 @pytest.mark.parametrize("R,V,k", [(1, 1, 1), (3, 2, 1), (4, 33, 7), (2, 128, 128), (5, 1000, 100), (3, 32768, 64),
                                    (1, 32768, 20), (2, 50001, 33), (1, 131075, 128), (300, 515, 8), (2, 300001, 5),
-                                   (600, 2052, 16)])
+                                   (600, 2052, 16), (2700, 700, 100), (2700, 4001, 9), (2700, 40, 40)])
 def test_loss_and_gradient(R, V, k, tail, dtype):
     x = logits(R, V, dtype, R * 3 + V + k).cuda()
     # the whole vocabulary listed: the list is the teacher's whole distribution
@@ -200,6 +200,9 @@ def test_unused_slots_masks_and_repeated_ids(V, tail):
     mask = torch.ones(10, dtype=torch.bool)
     mask[3:5] = False
     check(x, ids, lp, tail=tail, row_mask=mask.cuda(), upstream=torch.arange(1.0, 11.0).cuda())
+    if V <= 4100:  # the same among many rows
+        check(x.repeat(270, 1), ids.repeat(270, 1), lp.repeat(270, 1), tail=tail, row_mask=mask.cuda().repeat(270),
+              upstream=torch.arange(1.0, 11.0).cuda().repeat(270))
 
 
 @pytest.mark.gpu

@@ -192,7 +192,7 @@ def test_c_entry_refuses_bad_arguments():
 # ------------------------------------------------------------------ GPU
 
 SHAPES = [(1, 1), (3, 2), (5, 31), (2, 129), (7, 1000), (4, 4097), (3, 32768), (1, 32768), (2, 50001), (9, 8192),
-          (300, 515), (1, 131075), (2, 300000), (700, 2049), (1, 1 << 20)]
+          (300, 515), (1, 131075), (2, 300000), (700, 2049), (1, 1 << 20), (2700, 601), (2700, 2049), (2700, 5), (2665, 8192)]
 
 
 @pytest.mark.gpu
@@ -213,7 +213,7 @@ def test_forward(R, V, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
-@pytest.mark.parametrize("R,V", [(6, 77), (3, 32768), (40, 8200), (2, 140001)])
+@pytest.mark.parametrize("R,V", [(6, 77), (3, 32768), (40, 8200), (2, 140001), (2700, 77), (2700, 2051)])
 @pytest.mark.parametrize("kind", ["equal", "two_values", "rising", "falling", "front", "stripe", "zeros_signed"])
 def test_top_order_of_hard_rows(R, V, dtype, kind):
     """Rows with many ties, and rows whose large values lie together: the ids are exact, ties to the lowest."""
@@ -225,9 +225,9 @@ def test_top_order_of_hard_rows(R, V, dtype, kind):
            "stripe": torch.where(i % 8 == 3, 5.0 + (i % 24) / 8, -1.0),
            "zeros_signed": torch.where(i % 3 == 0, 0.0, -0.0)}[kind]
     x = (row + torch.zeros(R, 1)).to(TYPES[dtype]).cuda()
-    for r in range(R):
+    for r in range(min(R, 40)):
         x[r] = x[r].roll(r * 11)
-    for k in sorted({1, min(7, V), min(64, V), min(128, V)}):
+    for k in sorted({1, min(7, V), min(32, V), min(64, V), min(128, V)}):
         check_forward(token_logprobs(x, top_k=k), x, None, k, 1.0)
 
 
@@ -260,6 +260,9 @@ def test_masked_and_special_rows(V, dtype):
     targets[2], targets[4] = 0, 2
     for k in (1, 20, min(50, V)):
         check_forward(token_logprobs(x, targets, top_k=k), x, targets, k, 1.0)
+    if V <= 4096:  # the same among many rows
+        many, more = x.repeat(180, 1), targets.repeat(180)
+        check_forward(token_logprobs(many, more, top_k=20), many, more, 20, 1.0)
     check_forward(token_logprobs(x[:6], targets[:6], top_k=3, temperature=4.0), x[:6], targets[:6], 3, 4.0)
 
 
@@ -280,7 +283,8 @@ def test_targets_outside_and_ignored():
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("R,V,k", [(1, 1, 1), (3, 2, 2), (5, 31, 4), (2, 129, 128), (6, 1000, 0), (3, 32768, 20),
-                                   (2, 50001, 3), (1, 131075, 8), (400, 519, 5), (1, 1 << 20, 2)])
+                                   (2, 50001, 3), (1, 131075, 8), (400, 519, 5), (1, 1 << 20, 2),
+                                   (2700, 601, 5), (2700, 4000, 0)])
 def test_gradient(R, V, k, dtype):
     from dwarf_v2_b200.logprobs import token_logprobs
 
