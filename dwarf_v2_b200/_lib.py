@@ -311,7 +311,7 @@ class TokenLogprobsBwdArgs(ctypes.Structure):
 class TopkDistillArgs(ctypes.Structure):
     _fields_ = _fields("""version:i32, dtype:i32, logits:ptr, outer:i64, inner:i64, vocab:i64, so:i64, si:i64,
         teacher_ids:ptr, teacher_logprobs:ptr, k:i32, tail:i32, row_mask:ptr, inv_temperature:f32,
-        grad_rows_stride:i32, grad_scale:ptr, grad_rows:ptr, loss:ptr, grad:ptr, skip_if_one:i32, loss_scale:f32, scale:f32""")
+        grad_rows_stride:i32, grad_scale:ptr, grad_rows:ptr, loss:ptr, grad:ptr, stats:ptr, skip_if_one:i32, loss_scale:f32, scale:f32""")
 
 
 class RowReduceArgs(ctypes.Structure):

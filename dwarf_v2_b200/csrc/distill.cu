@@ -21,14 +21,10 @@ __device__ __forceinline__ void warp_join(float c2, float& m, float& a, float& b
   b = warp_sum(b == 0.0f ? 0.0f : f * b);
 }
 
-// One CTA, or a cluster of them, for a row. With the gradient the row is read twice, the
-// second time from L2: one bulk prefetch at the start fetches the row while the teacher's list is
-// read, under a policy that keeps it there, and the threads of a CTA are chosen so that the
-// rows in flight are about 40 MB. 16384 rows of 32768 bf16, 64 entries: 388 us (128 threads
-// without either: 534, with 475 MB read for 268; the row held in shared memory: 483; 512
-// threads: 540). The loss alone: 128 threads, no prefetch, 196 us (256 threads: 249).
-template <typename T, int NT, bool kGrad>
-__device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, int cluster, int64_t r) {
+// One row, or a CTA's part of one. kKnown: the gradient from the sums that a launch with
+// the loss has left in `stats`; the parts need nothing of each other. Otherwise the CTAs of a row are a cluster.
+template <typename T, int NT, bool kGrad, bool kKnown>
+__device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, int parts, int rank, int64_t r) {
   using V = Vec16<T>;
   constexpr int kWarps = NT / 32, kTile = kVectors * NT;
   constexpr int kSlots = NT < DWARF_TOP_K_MAX ? DWARF_TOP_K_MAX / NT : 1;  // slots of the teacher's list for a thread
@@ -43,15 +39,16 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
   __shared__ int s_flags, s_listed;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int vocab = (int)a.vocab, k = a.k;
-  const int rank = cluster > 1 ? (int)cluster_rank() : 0;
+  const int cluster = kKnown ? 1 : parts;
   if (cluster > 1) cluster_arrive();  // its CTAs have started, before one writes to another
   const T* x = static_cast<const T*>(a.logits) + row_offset(r, a.inner, a.so, a.si);
-  const Part<T, NT> part(x, vocab, rank, cluster);
-  const uint64_t keep = kGrad ? policy_keep() : 0;
+  const Part<T, NT> part(x, vocab, rank, parts);
+  constexpr bool kTwice = kGrad && !kKnown;  // the row is read a second time, from L2
+  const uint64_t keep = kTwice ? policy_keep() : 0;
 
   // the teacher's slots
   const bool counted = a.row_mask == nullptr || a.row_mask[r] != 0;
-  if (kGrad && tid == 0 && counted) part.prefetch_kept(keep);
+  if (kTwice && tid == 0 && counted) part.prefetch_kept(keep);
   int id[kSlots];  // -1: not used; vocab: past the vocabulary
   float l[kSlots];
 #pragma unroll
@@ -67,7 +64,8 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
     }
   }
   const int words = ((part.j1 - part.j0) * V::kVec + 31) / 32;
-  for (int i = tid; i < words; i += NT) listed[i] = 0;
+  if (!kKnown)
+    for (int i = tid; i < words; i += NT) listed[i] = 0;
   bool any = false;
 #pragma unroll
   for (int s = 0; s < kSlots; ++s) {
@@ -88,7 +86,7 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
   float xv[kSlots];
 #pragma unroll
   for (int s = 0; s < kSlots; ++s) {
-    if (id[s] >= 0 && id[s] < vocab && part.holds(id[s])) {
+    if (!kKnown && id[s] >= 0 && id[s] < vocab && part.holds(id[s])) {
       const int at = id[s] + part.row.lead - part.j0 * V::kVec;
       const uint32_t bit = 1u << (at & 31);
       if (atomicOr(&listed[at >> 5], bit) & bit) atomicOr(&s_flags, 1);  // an id that another slot has too
@@ -120,100 +118,107 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
 
   const float c2 = a.inv_temperature * kLog2e;
   const float2 cc = make_float2(c2, c2);
-  float m = -CUDART_INF_F;
-  float2 sum = make_float2(0.0f, 0.0f), sum_list = sum;  // the ids not listed; those listed
-  for (int at = 0; at < part.size(); at += kTile) {
-    uint4 v[kVectors];
-    if (kGrad) part.load(at, v, keep); else part.load(at, v);
-    typename V::Max mv = V::max_of(v[0]);
+  float m = -CUDART_INF_F, s_r, s_l, rest = 0.0f;  // maximum, sums over the ids not listed and those listed
+  if (!kKnown) {
+    float2 sum = make_float2(0.0f, 0.0f), sum_list = sum;
+    for (int at = 0; at < part.size(); at += kTile) {
+      uint4 v[kVectors];
+      if (kTwice) part.load(at, v, keep); else part.load(at, v);
+      typename V::Max mv = V::max_of(v[0]);
 #pragma unroll
-    for (int i = 1; i < kVectors; ++i) mv = V::join(mv, V::max_of(v[i]));
-    const float m_new = fmaxf(m, warp_max(V::largest(mv)));
-    if (m > -CUDART_INF_F) {  // a later tile: move the sums to the new maximum
-      const float f = ex2_approx((m - m_new) * c2);
-      sum = mul2(sum, make_float2(f, f));
-      sum_list = mul2(sum_list, make_float2(f, f));
-    }
-    m = m_new;
-    const float s = m == -CUDART_INF_F ? 0.0f : -m;
-    // the bits of a thread's vectors of a tile lie NT kVec / 8 bytes apart
-    const int place = part.w0 - part.j0 + at + tid;
-    const unsigned char* bits = reinterpret_cast<const unsigned char*>(listed) + place * V::kVec / 8;
-    const int bits_shift = V::kVec == 4 ? 4 * (place & 1) : 0;
-    auto add = [&](const uint4& w, uint32_t mask) {
-      float2 e[V::kVec / 2];
-      V::unpack(w, e);
-#pragma unroll
-      for (int h = 0; h < V::kVec / 2; ++h) {
-        const float2 d = mul2(add2(e[h], make_float2(s, s)), cc);
-        e[h] = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+      for (int i = 1; i < kVectors; ++i) mv = V::join(mv, V::max_of(v[i]));
+      const float m_new = fmaxf(m, warp_max(V::largest(mv)));
+      if (m > -CUDART_INF_F) {  // a later tile: move the sums to the new maximum
+        const float f = ex2_approx((m - m_new) * c2);
+        sum = mul2(sum, make_float2(f, f));
+        sum_list = mul2(sum_list, make_float2(f, f));
       }
-      if (mask != 0) {
+      m = m_new;
+      const float s = m == -CUDART_INF_F ? 0.0f : -m;
+      // the bits of a thread's vectors of a tile lie NT kVec / 8 bytes apart
+      const int place = part.w0 - part.j0 + at + tid;
+      const unsigned char* bits = reinterpret_cast<const unsigned char*>(listed) + place * V::kVec / 8;
+      const int bits_shift = V::kVec == 4 ? 4 * (place & 1) : 0;
+      auto add = [&](const uint4& w, uint32_t mask) {
+        float2 e[V::kVec / 2];
+        V::unpack(w, e);
 #pragma unroll
         for (int h = 0; h < V::kVec / 2; ++h) {
-          if (mask & (1u << (2 * h))) sum_list.x += e[h].x, e[h].x = 0.0f;
-          if (mask & (2u << (2 * h))) sum_list.y += e[h].y, e[h].y = 0.0f;
+          const float2 d = mul2(add2(e[h], make_float2(s, s)), cc);
+          e[h] = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+        }
+        if (mask != 0) {
+#pragma unroll
+          for (int h = 0; h < V::kVec / 2; ++h) {
+            if (mask & (1u << (2 * h))) sum_list.x += e[h].x, e[h].x = 0.0f;
+            if (mask & (2u << (2 * h))) sum_list.y += e[h].y, e[h].y = 0.0f;
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < V::kVec / 2; ++h) sum = add2(sum, e[h]);
+      };
+      if (at + kTile <= part.size()) {
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i)
+          add(v[i], (bits[i * NT * V::kVec / 8] >> bits_shift) & ((1u << V::kVec) - 1u));
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+          if (at + i * NT >= part.size()) break;
+          const bool in = at + i * NT + tid < part.size();  // vectors outside hold -inf
+          add(v[i], in ? (bits[i * NT * V::kVec / 8] >> bits_shift) & ((1u << V::kVec) - 1u) : 0u);
         }
       }
-#pragma unroll
-      for (int h = 0; h < V::kVec / 2; ++h) sum = add2(sum, e[h]);
-    };
-    if (at + kTile <= part.size()) {
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i)
-        add(v[i], (bits[i * NT * V::kVec / 8] >> bits_shift) & ((1u << V::kVec) - 1u));
-    } else {
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i) {
-        if (at + i * NT >= part.size()) break;
-        const bool in = at + i * NT + tid < part.size();  // vectors outside hold -inf
-        add(v[i], in ? (bits[i * NT * V::kVec / 8] >> bits_shift) & ((1u << V::kVec) - 1u) : 0u);
-      }
     }
-  }
-  if (warp == 0 && part.ends()) {
-    const float m_new = fmaxf(m, warp_max(end)), base = m_new == -CUDART_INF_F ? 0.0f : m_new;
-    const float f = ex2_approx((m - base) * c2), e = ex2_approx((end - base) * c2);
-    sum = mul2(sum, make_float2(f, f));
-    sum_list = mul2(sum_list, make_float2(f, f));
-    const int at = end_id + part.row.lead - part.j0 * V::kVec;
-    if (end_id >= 0 && ((listed[at >> 5] >> (at & 31)) & 1u)) sum_list.x += e; else sum.x += e;
-    m = m_new;
-  }
-  float s_r = warp_sum(sum.x + sum.y), s_l = warp_sum(sum_list.x + sum_list.y);
-  if (lane == 0) s_m[warp] = m, s_rest[warp] = s_r, s_list[warp] = s_l;
-  if (k >= vocab) {  // every id may be listed: nothing is left to be the rest
-    for (int i = tid; i < words; i += NT) atomicAdd(&s_listed, __popc(listed[i]));
-  }
-  __syncthreads();
-  // every warp joins the warps' sums, then the parts' sums, in the same order
-  s_r = lane < kWarps ? s_rest[lane] : 0.0f;
-  s_l = lane < kWarps ? s_list[lane] : 0.0f;
-  m = lane < kWarps ? s_m[lane] : -CUDART_INF_F;
-  warp_join(c2, m, s_r, s_l);
-  if (cluster > 1) {
-    if (tid < 3 * cluster)
-      st_cluster(cluster_address(&s_parts[rank][tid % 3], tid / 3), tid % 3 == 0 ? m : tid % 3 == 1 ? s_r : s_l);
-    cluster_arrive();
-    cluster_wait();
-    m = lane < cluster ? s_parts[lane][0] : -CUDART_INF_F;
-    s_r = lane < cluster ? s_parts[lane][1] : 0.0f;
-    s_l = lane < cluster ? s_parts[lane][2] : 0.0f;
+    if (warp == 0 && part.ends()) {
+      const float m_new = fmaxf(m, warp_max(end)), base = m_new == -CUDART_INF_F ? 0.0f : m_new;
+      const float f = ex2_approx((m - base) * c2), e = ex2_approx((end - base) * c2);
+      sum = mul2(sum, make_float2(f, f));
+      sum_list = mul2(sum_list, make_float2(f, f));
+      const int at = end_id + part.row.lead - part.j0 * V::kVec;
+      if (end_id >= 0 && ((listed[at >> 5] >> (at & 31)) & 1u)) sum_list.x += e; else sum.x += e;
+      m = m_new;
+    }
+    s_r = warp_sum(sum.x + sum.y);
+    s_l = warp_sum(sum_list.x + sum_list.y);
+    if (lane == 0) s_m[warp] = m, s_rest[warp] = s_r, s_list[warp] = s_l;
+    if (k >= vocab) {  // every id may be listed: nothing is left to be the rest
+      for (int i = tid; i < words; i += NT) atomicAdd(&s_listed, __popc(listed[i]));
+    }
+    __syncthreads();
+    // every warp joins the warps' sums, then the parts' sums, in the same order
+    s_r = lane < kWarps ? s_rest[lane] : 0.0f;
+    s_l = lane < kWarps ? s_list[lane] : 0.0f;
+    m = lane < kWarps ? s_m[lane] : -CUDART_INF_F;
     warp_join(c2, m, s_r, s_l);
+    if (cluster > 1) {
+      if (tid < 3 * cluster)
+        st_cluster(cluster_address(&s_parts[rank][tid % 3], tid / 3), tid % 3 == 0 ? m : tid % 3 == 1 ? s_r : s_l);
+      cluster_arrive();
+      cluster_wait();
+      m = lane < cluster ? s_parts[lane][0] : -CUDART_INF_F;
+      s_r = lane < cluster ? s_parts[lane][1] : 0.0f;
+      s_l = lane < cluster ? s_parts[lane][2] : 0.0f;
+      warp_join(c2, m, s_r, s_l);
+    }
+    if (m == -CUDART_INF_F) m = 0.0f;
+  } else {
+    const float4 known = reinterpret_cast<const float4*>(a.stats)[r];
+    m = known.x, s_r = known.y, s_l = known.z, rest = known.w;
   }
-  if (m == -CUDART_INF_F) m = 0.0f;
   const float total = s_r + s_l;
   // the teacher: log p of the slot, sum p + rest, the rest
   const bool off = s_flags & 2;
-  float weight = 1.0f, rest = 0.0f;
+  float weight = 1.0f;
   if (a.tail) {
     double sum_p = 0.0;
 #pragma unroll
     for (int w = 0; w < kListWarps; ++w) sum_p += s_sum[w];
-    rest = (float)fmax(0.0, 1.0 - sum_p);
-    if (s_listed == vocab) rest = 0.0f;
+    if (!kKnown) {
+      rest = s_listed == vocab ? 0.0f : (float)fmax(0.0, 1.0 - sum_p);
+      if (sum_p != sum_p) rest = CUDART_NAN_F;
+    }
     weight = (float)(sum_p + (double)rest);
-    if (sum_p != sum_p) rest = weight = CUDART_NAN_F;
   } else {
     float top = -CUDART_INF_F, sum_p = 0.0f;
 #pragma unroll
@@ -250,7 +255,7 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
     const uint64_t leave = policy_leave();
     for (int at = 0; at < part.size(); at += kTile) {
       uint4 v[kVectors];
-      part.load(at, v, leave);
+      if (kTwice) part.load(at, v, leave); else part.load(at, v);
       store.tile(part, at, v, [&](const uint4& w) {
         float2 e[V::kVec / 2];
         V::unpack(w, e);
@@ -270,7 +275,7 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
     for (int s = 0; s < kSlots; ++s) {
       if (id[s] < 0 || id[s] >= vocab || !part.holds(id[s])) continue;
       float taken = p[s];
-      if (s_flags & 1) {
+      if (kKnown || (s_flags & 1)) {
         taken = 0.0f;
         for (int j = 0; j < k; ++j)
           if (s_id[j] == id[s]) taken += s_p[j];
@@ -284,22 +289,30 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
     for (int w = 0; w < kListWarps; ++w) term += s_term[w];
     if (!(rest <= 0.0f)) term += rest * (logf(rest) - log2f(s_r) * kLn2 + ln_total);
     a.loss[r] = off ? CUDART_NAN_F : term * a.loss_scale;
+    if (a.stats != nullptr) reinterpret_cast<float4*>(a.stats)[r] = make_float4(m, s_r, s_l, rest);
   }
 }
 
+// The loss, and with kGrad the gradient in the same launch: the row is then read twice, the
+// second time from L2. One bulk prefetch at the start fetches the row while the teacher's list
+// is read, under a policy that keeps it there, and the threads of a CTA are chosen so that the
+// rows in flight are about 40 MB. 16384 rows of 32768 bf16, 64 entries: 383 us (128 threads
+// without either: 534, with 475 MB read for 268; the row held in shared memory: 483; 512
+// threads: 540). The loss alone: 128 threads, no prefetch, 196 us (256 threads: 249).
 template <typename T, int NT, bool kGrad>
 __global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_kernel(const dwarf_topk_distill_args a, int cluster) {
-  if (a.skip_if_one && *a.grad_rows == 1.0f) return;
-  distill_row<T, NT, kGrad>(a, cluster, blockIdx.x / (unsigned)cluster);
+  const int rank = cluster > 1 ? (int)cluster_rank() : 0;
+  distill_row<T, NT, kGrad, false>(a, cluster, rank, blockIdx.x / (unsigned)cluster);
 }
 
-// The gradient anew where the upstream gradient is not 1: a grid of one wave, which costs 3 us
-// (a CTA for each of 16384 rows: 11 us) where there is nothing to do.
+// The gradient from the sums of an earlier launch. With skip_if_one a grid of one wave, which
+// costs 3 us (a CTA for each of 16384 rows: 11 us) where there is nothing to do.
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_again_kernel(const dwarf_topk_distill_args a) {
-  if (*a.grad_rows == 1.0f) return;
-  for (int64_t r = blockIdx.x; r < a.outer * a.inner; r += gridDim.x) {
-    distill_row<T, NT, true>(a, 1, r);
+__global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_grad_kernel(const dwarf_topk_distill_args a, int parts) {
+  if (a.skip_if_one && *a.grad_rows == 1.0f) return;
+  const uint32_t n = (uint32_t)(a.outer * a.inner) * (uint32_t)parts;
+  for (uint32_t i = blockIdx.x; i < n; i += gridDim.x) {
+    distill_row<T, NT, true, true>(a, parts, (int)(i % (uint32_t)parts), i / (uint32_t)parts);
     __syncthreads();  // before the next row's list takes this one's place
   }
 }
@@ -334,25 +347,27 @@ template <typename T>
 int launch_distill(const dwarf_topk_distill_args& a, cudaStream_t stream) {
   const int64_t rows = a.outer * a.inner;
   const int vectors = ceil_div((int)a.vocab, Vec16<T>::kVec);
+  // 32768 rows of 4096 bf16: 226 us with 128 threads, 137 with a warp; 16384 of 4096 fp32: 111, 129
+  const bool warps = warp_rows(rows, vectors, a.grad == nullptr ? 2048 : 512);
+  if (a.loss == nullptr) {
+    const int parts = warps ? 1 : parts_for(rows, vectors), threads = warps ? 32 : 128;
+    int64_t grid = rows * parts;
+    if (a.skip_if_one && grid > kNumSMs * (1024 / threads)) grid = kNumSMs * (1024 / threads);
+    return launch_rows(warps ? topk_distill_grad_kernel<T, 32> : topk_distill_grad_kernel<T, 128>, grid, 1, threads, 0,
+                       stream, a, parts);
+  }
   const int cluster = cluster_for(rows, vectors, 262144 / Vec16<T>::kVec);  // a bit for each place: at most 32 KB
   // a row that starts off a 16-byte boundary has one vector more
   const int part = ceil_div(vectors + 1, cluster);
   const int bytes = (part * Vec16<T>::kVec + 31) / 32 * 4;
-  if (a.grad == nullptr && warp_rows(rows, vectors, 2048))
-    return launch_rows(topk_distill_kernel<T, 32, false>, rows, 1, 32, bytes, stream, a, 1);
-  if (a.grad == nullptr)
-    return launch_rows(topk_distill_kernel<T, 128, false>, rows, cluster, 128, bytes, stream, a, cluster);
-  const auto go = [&](auto kernel, auto again, int threads) {
-    // the same split of a row either way: the same bits
-    if (!a.skip_if_one || cluster > 1) return launch_rows(kernel, rows, cluster, threads, bytes, stream, a, cluster);
-    const int64_t wave = (int64_t)kNumSMs * (1024 / threads);
-    return launch_rows(again, rows < wave ? rows : wave, 1, threads, bytes, stream, a);
+  const auto go = [&](auto kernel, int threads) {
+    return launch_rows(kernel, rows, cluster, threads, bytes, stream, a, cluster);
   };
-  // 32768 rows of 4096 bf16: 226 us with 128 threads, 137 with a warp; 16384 of 4096 fp32: 111, 129
-  if (warp_rows(rows, vectors, 512)) return go(topk_distill_kernel<T, 32, true>, topk_distill_again_kernel<T, 32>, 32);
-  if (part <= 2048) return go(topk_distill_kernel<T, 128, true>, topk_distill_again_kernel<T, 128>, 128);
-  if (part <= 4097) return go(topk_distill_kernel<T, 256, true>, topk_distill_again_kernel<T, 256>, 256);
-  return go(topk_distill_kernel<T, 512, true>, topk_distill_again_kernel<T, 512>, 512);
+  if (a.grad == nullptr) return warps ? go(topk_distill_kernel<T, 32, false>, 32) : go(topk_distill_kernel<T, 128, false>, 128);
+  if (warps) return go(topk_distill_kernel<T, 32, true>, 32);
+  if (part <= 2048) return go(topk_distill_kernel<T, 128, true>, 128);
+  if (part <= 4097) return go(topk_distill_kernel<T, 256, true>, 256);
+  return go(topk_distill_kernel<T, 512, true>, 512);
 }
 
 }  // namespace
@@ -370,7 +385,8 @@ extern "C" int dwarf_topk_distill(const dwarf_topk_distill_args* args, void* str
   if (a.skip_if_one && (a.grad_rows == nullptr || a.grad_rows_stride != 0 || a.loss != nullptr)) return DWARF_ERR_VALUE;
   if (a.outer * a.inner == 0) return DWARF_OK;
   if (a.teacher_ids == nullptr || a.teacher_logprobs == nullptr) return DWARF_ERR_NULL;
-  if (a.loss == nullptr && a.grad == nullptr) return DWARF_ERR_NULL;
+  if (a.loss == nullptr && (a.grad == nullptr || a.stats == nullptr)) return DWARF_ERR_NULL;
+  if (!aligned16(a.stats)) return DWARF_ERR_ALIGN;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a.dtype == DWARF_F32) return launch_distill<float>(a, s);
   if (a.dtype == DWARF_BF16) return launch_distill<__nv_bfloat16>(a, s);

@@ -10,8 +10,8 @@ kernel (``dwarf_topk_distill`` in the C ABI).
 Where the loss is reduced (``"mean"``, ``"sum"``) and the logits require grad,
 the forward launch writes the gradient for an upstream gradient of 1 in the same
 pass over the logits; backward's launch leaves it as it is when the upstream
-gradient is 1, and otherwise computes it anew from the logits (one rounding
-either way). ``weight`` scales the loss without leaving the one-pass form.
+gradient is 1, and otherwise computes it anew from the logits and the sums that the
+forward launch has left (one rounding either way). ``weight`` scales the loss without leaving the one-pass form.
 """
 
 from __future__ import annotations
@@ -26,7 +26,7 @@ from . import _lib, _rows
 __all__ = ["TopKDistillationLoss", "topk_distillation_loss"]
 
 
-def _launch(logits, ids, logprobs, mask, inv_temperature, tail, *, loss=None, grad=None, grad_scale=None,
+def _launch(logits, ids, logprobs, mask, inv_temperature, tail, *, loss=None, grad=None, stats=None, grad_scale=None,
             grad_rows=None, skip_if_one=False, loss_scale=1.0, scale=1.0) -> None:
     logits, outer, inner, so, si = _rows.addressed(logits)
     args = _lib.TopkDistillArgs(
@@ -35,7 +35,7 @@ def _launch(logits, ids, logprobs, mask, inv_temperature, tail, *, loss=None, gr
         teacher_logprobs=logprobs.data_ptr(), k=ids.shape[-1], tail=int(tail), row_mask=_lib.ptr(mask),
         inv_temperature=inv_temperature, grad_rows_stride=int(grad_rows is not None and grad_rows.ndim > 0),
         grad_scale=_lib.ptr(grad_scale), grad_rows=_lib.ptr(grad_rows), loss=_lib.ptr(loss), grad=_lib.ptr(grad),
-        skip_if_one=int(skip_if_one), loss_scale=loss_scale, scale=scale)
+        stats=_lib.ptr(stats), skip_if_one=int(skip_if_one), loss_scale=loss_scale, scale=scale)
     if outer * inner:
         _rows.launch("dwarf_topk_distill", args, logits.device)
 
@@ -50,26 +50,26 @@ def _reduce(out, *, values=None, mask=None, host_scale=1.0) -> None:
 class _TopKDistillationFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, logprobs, mask, inv_temperature, tail, reduction, weight):
-        ctx.save_for_backward(logits, ids, logprobs, mask)
+        stats = torch.empty(*logits.shape[:-1], 4, dtype=torch.float32, device=logits.device)
+        ctx.save_for_backward(logits, ids, logprobs, mask, stats)
         ctx.scalars = (inv_temperature, tail)
         ctx.grad = None
-        ctx.scale, ctx.grad_scale = weight, None
         if reduction != "none":
             ctx.grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         loss, ctx.scale, ctx.grad_scale = _forward(logits, ids, logprobs, mask, inv_temperature, tail, reduction,
-                                                   weight, ctx.grad)
+                                                   weight, ctx.grad, stats)
         return loss
 
     @staticmethod
     def backward(ctx, g):
         if torch.is_grad_enabled():  # create_graph: a second derivative is refused, not left out
             return _once_more(ctx, g)
-        logits, ids, logprobs, mask = ctx.saved_tensors
+        logits, ids, logprobs, mask, stats = ctx.saved_tensors
         grad, ctx.grad = ctx.grad, None  # a second backward gets a buffer of its own
         written = grad is not None
         if not written:
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _launch(logits, ids, logprobs, mask, *ctx.scalars, grad=grad, grad_scale=ctx.grad_scale,
+        _launch(logits, ids, logprobs, mask, *ctx.scalars, grad=grad, stats=stats, grad_scale=ctx.grad_scale,
                 grad_rows=g.contiguous(), skip_if_one=written, scale=ctx.scale)
         return grad, None, None, None, None, None, None, None
 
@@ -77,7 +77,7 @@ class _TopKDistillationFn(torch.autograd.Function):
 _once_more = torch.autograd.function.once_differentiable(_TopKDistillationFn.backward)
 
 
-def _forward(logits, ids, logprobs, mask, inv_temperature, tail, reduction, weight, grad):
+def _forward(logits, ids, logprobs, mask, inv_temperature, tail, reduction, weight, grad=None, stats=None):
     """(loss, host and device factors of the gradient)."""
     dev = logits.device
     rows = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
@@ -87,10 +87,10 @@ def _forward(logits, ids, logprobs, mask, inv_temperature, tail, reduction, weig
     if reduction == "mean":
         if mask is None:
             scale = weight / rows.numel()
-        elif grad is not None:  # the gradient needs the number of rows before the loss is there
+        elif stats is not None:  # the gradient needs the number of rows before the loss is there
             grad_scale = torch.empty((), dtype=torch.float32, device=dev)
             _reduce(grad_scale, mask=mask)
-    _launch(logits, ids, logprobs, mask, inv_temperature, tail, loss=rows, grad=grad, grad_scale=grad_scale,
+    _launch(logits, ids, logprobs, mask, inv_temperature, tail, loss=rows, grad=grad, stats=stats, grad_scale=grad_scale,
             loss_scale=weight, scale=scale)
     if reduction == "none":
         return rows, scale, grad_scale
@@ -156,8 +156,7 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teac
     if grad and logits.requires_grad:
         return _TopKDistillationFn.apply(logits, teacher_ids, teacher_logprobs, row_mask, inv_temperature, bool(tail),
                                          reduction, weight)
-    return _forward(logits, teacher_ids, teacher_logprobs, row_mask, inv_temperature, bool(tail), reduction, weight,
-                    None)[0]
+    return _forward(logits, teacher_ids, teacher_logprobs, row_mask, inv_temperature, bool(tail), reduction, weight)[0]
 
 
 class TopKDistillationLoss(nn.Module):

@@ -813,8 +813,10 @@ int dwarf_token_logprobs_bwd(const dwarf_token_logprobs_bwd_args* args, void* st
  * logits not used.
  *   grad_v = s c (q_v (sum p + p_*) - sum over slots with id v of p - [v not listed] p_* q_v / q_*)
  * where s = scale * (grad_scale ? *grad_scale : 1) * (grad_rows ? grad_rows[row or 0] : 1).
- * With skip_if_one the launch leaves grad as it is when grad_rows[0] == 1 (the
- * gradient that the forward launch has written stands). */
+ * A launch for the gradient alone reads the row once, with the sums that the
+ * launch with the loss has left in stats. With skip_if_one it leaves grad as it
+ * is when grad_rows[0] == 1 (the gradient that the forward launch has written
+ * stands). */
 typedef struct {
   int32_t version;
   int32_t dtype;                  /* of logits and grad                    */
@@ -830,8 +832,11 @@ typedef struct {
   int32_t grad_rows_stride;       /* 0: one scalar, 1: one per row         */
   const float* grad_scale;        /* optional device scalar                */
   const float* grad_rows;         /* optional device scalar or [rows]      */
-  float* loss;                    /* optional [rows]                       */
+  float* loss;                    /* [rows]; NULL: the gradient alone      */
   void* grad;                     /* optional [rows, vocab], contiguous    */
+  float* stats;                   /* optional float4 [rows], 16-byte
+                                     aligned: written with the loss; read
+                                     (and required) for the gradient alone */
   int32_t skip_if_one;            /* with grad_rows, stride 0, no loss     */
   float loss_scale;               /* factor of loss                        */
   float scale;                    /* factor of grad                        */

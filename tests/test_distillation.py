@@ -156,6 +156,7 @@ def test_c_entry_refuses_bad_arguments():
     assert status(tail=2) == -9 and status(grad_rows_stride=2) == -9
     assert status(skip_if_one=1, loss=None, grad=4096) == -9
     assert status(skip_if_one=1, grad=4096, grad_rows=4096) == -9
+    assert status(loss=None, grad=4096) == -2 and status(stats=4104) == -5
     assert status(inner=0) == 0
     reduce = lambda **f: lib.dwarf_row_reduce(ctypes.byref(_lib.RowReduceArgs(version=1, **f)), None)  # noqa: E731
     assert reduce(rows=-1, out=4096) == -3
