@@ -175,6 +175,7 @@ __device__ __forceinline__ int best_entries(const Part<T, NT>& part, const typen
     int c = 0;
     part.walk([&](const uint4& w, int j, bool in) {
       if (in) part.elements(w, j, [&](float x, int) { c += order_key(x) >= from; });
+      return true;
     });
     c = __reduce_add_sync(0xffffffffu, c);
     __syncthreads();
@@ -198,11 +199,12 @@ __device__ __forceinline__ int best_entries(const Part<T, NT>& part, const typen
       part.elements(w, j, [&](float x, int id) {
         if (order_key(x) > limit) sh.candidate[atomicAdd(&sh.n, 1)] = entry_key(x, (uint32_t)id);  // fewer than k
       });
+    return true;
   });
   __syncthreads();
   int have = sh.n;
   part.walk([&](const uint4& w, int j, bool in) {
-    if (have >= k) return;  // the same for the whole block
+    if (have >= k) return false;
     int c = 0;
     if (in) part.elements(w, j, [&](float x, int) { c += order_key(x) == limit; });
     int at = c;
@@ -228,6 +230,7 @@ __device__ __forceinline__ int best_entries(const Part<T, NT>& part, const typen
       });
     have = min(k, have + total);
     __syncthreads();
+    return true;
   });
   __syncthreads();
   return have;

@@ -473,14 +473,15 @@ struct Part {
       if (u >= row.lead && u < row.end) f(e & 1 ? x[e / 2].y : x[e / 2].x, u - row.lead);
     }
   }
-  // f(vector, j, whether j is in the part), one step of the whole block after the other, in rising j.
+  // f(vector, j, whether j is in the part), one step of the whole block after the other, in
+  // rising j, the row's ends included, while f says (the same for all threads) to go on.
   template <typename F>
   __device__ __forceinline__ void walk(F f) const {
     for (int first = j0; first < j1; first += kThreads) {
       const int j = first + threadIdx.x;
       uint4 w = make_uint4(0, 0, 0, 0);
       if (j < j1) w = row.load(j);
-      f(w, j, j < j1);
+      if (!f(w, j, j < j1)) break;
     }
   }
 };

@@ -121,7 +121,8 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teac
     * A slot with an id below 0 is not used; an id >= V makes its row NaN; an id
       listed twice counts with both probabilities.
     * ``row_mask`` [...] bool: rows where it is False, and rows without a used slot,
-      have loss 0 and gradient exactly 0 whatever their logits hold.
+      have loss 0 and gradient exactly 0 whatever their logits hold. A NaN or +inf among
+      another row's logits makes its loss and gradient NaN.
     * ``reduction``: "mean" over the rows that ``row_mask`` keeps, "sum", or "none"
       ([...]). The loss is fp32; no factor temperature**2 is applied.
 

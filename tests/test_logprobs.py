@@ -66,7 +66,9 @@ def check_forward(out, x, targets, k, t, ignore_index=-100):
 def grad_tolerance(x, t, grad, size):
     V = x.shape[-1]
     d = torch.nan_to_num((x.double() - x.double().amax(-1, keepdim=True)) / t, neginf=0.0).abs()
-    tiny = 2.0 ** -24 if x.dtype == torch.float16 else 2.0 ** -120
+    # an exponential below 2^-126 counts as 0: a term q (G + gH (|log q| + H)) is then left out whole, at most
+    # 2^-126 (2 + 88 + 12) < 2^-119 of gradients whose c G and c gH are 2 and 1 (the others have no such terms)
+    tiny = 2.0 ** -24 if x.dtype == torch.float16 else 2.0 ** -119
     return size * (4 * rel_of(V) + d * 2.0 ** -21) + torch.finfo(x.dtype).eps / 2 * grad.abs() * 1.01 + tiny
 
 
@@ -380,6 +382,27 @@ def test_strides_and_alignment(dtype):
         flat = view.reshape(-1, V)
         want, size = oracle.token_logprobs_grad(flat, targets.reshape(-1), g_logprob=w.reshape(-1))
         close(grad.reshape(-1, V), want, grad_tolerance(flat, 1.0, want, size), name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_without_targets_and_extreme_temperatures(dtype):
+    """Entropy, lse and alternatives alone, with their gradients; temperatures far from 1."""
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    x = logits(5, 3001, dtype, 12).cuda().requires_grad_()
+    for t in (1e-4, 0.02, 1e3):
+        out = token_logprobs(x, top_k=4, temperature=t)
+        check_forward(out, x.detach(), None, 4, t)
+        gh, gt = torch.full((5,), 1.0 * t).cuda(), torch.full((5, 4), 0.5 * t).cuda()
+        grad, = torch.autograd.grad([out.entropy, out.top_logprobs], x, [gh, gt])
+        want, size = oracle.token_logprobs_grad(x.detach(), top_ids=out.top_ids, temperature=t, g_entropy=gh, g_top=gt)
+        close(grad, want, grad_tolerance(x.detach(), t, want, size), t)
+    out = token_logprobs(x)
+    assert out.logprob is None and out.top_ids is None
+    grad, = torch.autograd.grad(out.lse.sum(), x)
+    want, size = oracle.token_logprobs_grad(x.detach(), g_lse=torch.ones(5).cuda())
+    close(grad, want, grad_tolerance(x.detach(), 1.0, want, size))
 
 
 @pytest.mark.gpu
