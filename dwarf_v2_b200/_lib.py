@@ -315,7 +315,7 @@ class TopkDistillArgs(ctypes.Structure):
 
 
 class RowReduceArgs(ctypes.Structure):
-    _fields_ = _fields("""version:i32, rows:i64, values:ptr, mask:ptr, scale:ptr, host_scale:f32, out:ptr""")
+    _fields_ = _fields("""version:i32, rows:i64, values:ptr, mask:ptr, host_scale:f32, out:ptr""")
 
 
 _ENTRY_POINTS = {

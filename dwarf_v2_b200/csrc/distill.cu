@@ -338,7 +338,6 @@ __global__ void __launch_bounds__(1024) row_reduce_kernel(const dwarf_row_reduce
   count = __reduce_add_sync(0xffffffffu, some ? s_count[lane] : 0);
   if (lane != 0) return;
   double out = a.values != nullptr ? sum * (double)a.host_scale : 1.0;
-  if (a.scale != nullptr) out *= (double)*a.scale;
   if (a.mask != nullptr) out /= (double)max(count, 1);
   *a.out = (float)out;
 }

@@ -237,9 +237,12 @@ __device__ __forceinline__ int best_entries(const Part<T, NT>& part, const typen
 }
 
 // One CTA, or a cluster of them, for a row: one pass that keeps a running maximum, S
-// and T for each warp. Eight CTAs of 128 threads on an SM overlap one's loads with
-// another's sums and search; 512 threads that hold a whole row reached 4.0 of these
-// 6.4 TB/s (16384 rows of 32768 bf16, no alternatives).
+// and T for each warp, then (kTop) the search for the alternatives. Small CTAs overlap one's
+// loads with another's sums and search: 16384 rows of 32768 bf16 take 162 us without
+// alternatives (6.6 TB/s; 512 threads that hold a whole row in registers: 277), 183 with 5,
+// 214 with 64, 294 with 128. With alternatives what bounds it is the latency of the search's
+// steps, of which the reading of the cells under a full memory pipe is the longest (at 64: bound
+// 1.2 k cycles, cells 0.8 k, reading them 4 k, ranking 2.5 k of 30 k for a row).
 template <typename T, int NT, bool kTop, bool kAhead>
 __global__ void __launch_bounds__(NT, NT == 32 ? 32 : kTop ? 9 : 8)
     token_logprobs_kernel(const dwarf_token_logprobs_args a, int cluster, int lists_at, int64_t ahead) {
@@ -503,7 +506,8 @@ int launch_forward(const dwarf_token_logprobs_args& a, cudaStream_t stream) {
 
 // grad_v = c (sparse terms - q_v (G + gH (log q_v + H))): each CTA writes its part of the
 // row, then the listed entries of that part again with their terms. One read of the
-// logits, one write; q from the forward's m and S.
+// logits, one write; q from the forward's m and S. 16384 rows of 32768 bf16: 333 us, 6.4 TB/s:
+// memory bounds it.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT)
     token_logprobs_bwd_kernel(const dwarf_token_logprobs_bwd_args a, int parts) {
@@ -534,7 +538,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
     g += v;
     any |= v != 0.0f;
   }
-  g = n > 1 ? block_reduce<NT>(g, sf, AddOp()) : g_lp;
+  g = n > 1 ? block_sum<NT>(g, sf) : g_lp;
   const float g_lse = a.g_lse != nullptr ? a.g_lse[r] : 0.0f;
   const float g_h = a.g_entropy != nullptr ? a.g_entropy[r] : 0.0f;
   any = __syncthreads_or(any) || g_lse != 0.0f || g_h != 0.0f;
@@ -612,6 +616,7 @@ extern "C" int dwarf_token_logprobs(const dwarf_token_logprobs_args* args, void*
   const int64_t rows = a.outer * a.inner;
   if (rows == 0) return DWARF_OK;
   if (a.lse == nullptr || a.entropy == nullptr) return DWARF_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(a.stats) & 7) return DWARF_ERR_ALIGN;
   if ((a.targets == nullptr) != (a.logprob == nullptr)) return DWARF_ERR_NULL;
   if (a.top_k > 0 && (a.top_logprobs == nullptr || a.top_ids == nullptr)) return DWARF_ERR_NULL;
   return with_type(a.dtype, [&](auto t) { return launch_forward<decltype(t)>(a, static_cast<cudaStream_t>(stream)); });
@@ -627,6 +632,7 @@ extern "C" int dwarf_token_logprobs_bwd(const dwarf_token_logprobs_bwd_args* arg
   const int64_t rows = a.outer * a.inner;
   if (rows == 0) return DWARF_OK;
   if (a.stats == nullptr || a.entropy == nullptr || a.grad == nullptr) return DWARF_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(a.stats) & 7) return DWARF_ERR_ALIGN;
   if (a.g_logprob != nullptr && a.targets == nullptr) return DWARF_ERR_NULL;
   if (a.g_top != nullptr && (a.top_ids == nullptr || a.top_k < 1)) return DWARF_ERR_NULL;
   return with_type(a.dtype, [&](auto t) { return launch_backward<decltype(t)>(a, static_cast<cudaStream_t>(stream)); });

@@ -1,5 +1,10 @@
 // Helpers of the vocabulary-row kernels (token log probabilities, distillation):
-// addressing of logit rows, conversions, the order of values, block reductions.
+// addressing of logit rows, conversions and packed operations, the order of values, a CTA's
+// part of a row, clusters, and the rules that split rows over CTAs.
+//
+// A row is read as 16-byte vectors from its first boundary on; a thread has eight of them in
+// flight. All sums are fp32, relative to a running maximum of each warp, and joined in a
+// fixed order (the same bits every time, for one split of the rows).
 #pragma once
 
 #include "common.cuh"
@@ -45,29 +50,18 @@ __device__ __forceinline__ uint64_t entry_key(float v, uint32_t id) {
 }
 __device__ __forceinline__ uint32_t entry_id(uint64_t key) { return ~(uint32_t)key; }
 
-// Sums (and maxima) over a block in a fixed order; every thread gets the result.
-// `scratch` holds one value per warp; a barrier at each end makes it reusable.
-template <int kThreads, typename V, typename F>
-__device__ __forceinline__ V block_reduce(V v, V* scratch, F f) {
+// The sum over a block, in a fixed order, for every thread. `scratch`: one value per warp.
+template <int kThreads>
+__device__ __forceinline__ float block_sum(float v, float* scratch) {
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
+  for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
   __syncthreads();
-  V t = scratch[0];
+  float t = scratch[0];
 #pragma unroll
-  for (int i = 1; i < kThreads / 32; ++i) t = f(t, scratch[i]);
+  for (int i = 1; i < kThreads / 32; ++i) t += scratch[i];
   return t;
 }
-
-struct AddOp {
-  template <typename V>
-  __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
-};
-struct MaxOp {
-  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
-  __device__ __forceinline__ uint64_t operator()(uint64_t a, uint64_t b) const { return a > b ? a : b; }
-};
 
 // Pairs of fp32: one issue slot for two elements.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }

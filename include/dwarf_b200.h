@@ -763,8 +763,8 @@ typedef struct {
   float* logprob;                 /* [rows] (with targets)                 */
   float* entropy;                 /* [rows]                                */
   float* lse;                     /* [rows]                                */
-  float* stats;                   /* optional float2 [rows]: (m, S), what
-                                     dwarf_token_logprobs_bwd reads        */
+  float* stats;                   /* optional float2 [rows], 8-byte aligned:
+                                     (m, S), what the gradient reads       */
   float* top_logprobs;            /* [rows, top_k]                         */
   int64_t* top_ids;               /* [rows, top_k]                         */
 } dwarf_token_logprobs_args;
@@ -845,14 +845,13 @@ typedef struct {
 int dwarf_topk_distill(const dwarf_topk_distill_args* args, void* stream);
 
 /* One fp32 value from rows, summed in 64 bits in a fixed order:
- *   out = [values: host_scale * sum of values; else 1] * [scale: *scale] / [mask: max(1, mask bytes set)]
+ *   out = [values: host_scale * sum of values; else 1] / [mask: max(1, mask bytes set)]
  * the reduced loss, or (without values) the scale of a mean over the rows that count. */
 typedef struct {
   int32_t version;
   int64_t rows;
   const float* values;            /* optional [rows]                       */
   const uint8_t* mask;            /* optional [rows]                       */
-  const float* scale;             /* optional device scalar                */
   float host_scale;
   float* out;                     /* [1]                                   */
 } dwarf_row_reduce_args;
