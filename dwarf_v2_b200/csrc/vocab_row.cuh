@@ -104,6 +104,11 @@ struct Vec16<float> {
   __device__ __forceinline__ static float value(const uint4& v, int e) {
     return __uint_as_float(e & 2 ? (e & 1 ? v.w : v.z) : (e & 1 ? v.y : v.x));
   }
+  // v without the elements of a mask (bit e: element e): -inf in their places.
+  __device__ __forceinline__ static uint4 drop(const uint4& v, uint32_t mask) {
+    return make_uint4(mask & 1u ? kMinusInf : v.x, mask & 2u ? kMinusInf : v.y, mask & 4u ? kMinusInf : v.z,
+                      mask & 8u ? kMinusInf : v.w);
+  }
   // Elements no lower than `low`.
   using Low = float;
   __device__ __forceinline__ static Low low_of(float v) { return v; }
@@ -177,6 +182,13 @@ struct Vec16<__nv_bfloat16> {
     const uint32_t w = e & 4 ? (e & 2 ? v.w : v.z) : (e & 2 ? v.y : v.x);
     return to_f32(__ushort_as_bfloat16((unsigned short)(e & 1 ? w >> 16 : w & 0xffffu)));
   }
+  __device__ __forceinline__ static uint32_t drop2(uint32_t w, uint32_t mask) {
+    const uint32_t gone = (mask & 1u ? 0x0000ffffu : 0u) | (mask & 2u ? 0xffff0000u : 0u);
+    return (w & ~gone) | (kMinusInf & gone);
+  }
+  __device__ __forceinline__ static uint4 drop(const uint4& v, uint32_t mask) {
+    return make_uint4(drop2(v.x, mask), drop2(v.y, mask >> 2), drop2(v.z, mask >> 4), drop2(v.w, mask >> 6));
+  }
   using Low = __nv_bfloat162;
   __device__ __forceinline__ static Low low_of(float v) { return __float2bfloat162_rn(v); }
   __device__ __forceinline__ static float low_value(Low low) { return __low2float(low); }
@@ -248,6 +260,13 @@ struct Vec16<__half> {
   __device__ __forceinline__ static float value(const uint4& v, int e) {
     const uint32_t w = e & 4 ? (e & 2 ? v.w : v.z) : (e & 2 ? v.y : v.x);
     return to_f32(__ushort_as_half((unsigned short)(e & 1 ? w >> 16 : w & 0xffffu)));
+  }
+  __device__ __forceinline__ static uint32_t drop2(uint32_t w, uint32_t mask) {
+    const uint32_t gone = (mask & 1u ? 0x0000ffffu : 0u) | (mask & 2u ? 0xffff0000u : 0u);
+    return (w & ~gone) | (kMinusInf & gone);
+  }
+  __device__ __forceinline__ static uint4 drop(const uint4& v, uint32_t mask) {
+    return make_uint4(drop2(v.x, mask), drop2(v.y, mask >> 2), drop2(v.z, mask >> 4), drop2(v.w, mask >> 6));
   }
   using Low = __half2;
   __device__ __forceinline__ static Low low_of(float v) { return __float2half2_rn(v); }

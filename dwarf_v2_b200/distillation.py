@@ -50,7 +50,7 @@ def _reduce(out, *, values=None, mask=None, host_scale=1.0) -> None:
 class _TopKDistillationFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, logprobs, mask, inv_temperature, tail, reduction, weight):
-        stats = torch.empty(*logits.shape[:-1], 4, dtype=torch.float32, device=logits.device)
+        stats = torch.empty(*logits.shape[:-1], 8, dtype=torch.float32, device=logits.device)
         ctx.save_for_backward(logits, ids, logprobs, mask, stats)
         ctx.scalars = (inv_temperature, tail)
         ctx.grad = None

@@ -834,9 +834,9 @@ typedef struct {
   const float* grad_rows;         /* optional device scalar or [rows]      */
   float* loss;                    /* [rows]; NULL: the gradient alone      */
   void* grad;                     /* optional [rows, vocab], contiguous    */
-  float* stats;                   /* optional float4 [rows], 16-byte
-                                     aligned: written with the loss; read
-                                     (and required) for the gradient alone */
+  float* stats;                   /* optional [rows, 8], 16-byte aligned:
+                                     written with the loss; read (and
+                                     required) for the gradient alone      */
   int32_t skip_if_one;            /* with grad_rows, stride 0, no loss     */
   float loss_scale;               /* factor of loss                        */
   float scale;                    /* factor of grad                        */

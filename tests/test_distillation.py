@@ -261,7 +261,10 @@ def test_masked_student(dtype):
         check(x[row:row + 1], ids[row:row + 1], lp[row:row + 1], tail=False)
     leaf = x.clone().requires_grad_()
     loss = topk_distillation_loss(leaf, ids, lp, reduction="none")
-    assert loss[0] == math.inf and loss[1] == math.inf and loss[3] == math.inf
+    assert loss[0] == math.inf and loss[3] == math.inf
+    want = oracle.topk_distillation(x[1:2], ids[1:2], lp[1:2])[0]  # a tenth of the lowest value: large, not inf
+    assert float(want) > 1e37
+    close(loss[1:2].detach(), want, 2.0 ** -20 * want.abs())
     grad, = torch.autograd.grad(loss, leaf, torch.ones(5, device="cuda"))
     assert torch.isfinite(grad[[2, 3, 4]]).all()
     close(grad[3, ids[3, 0]], -torch.exp(lp[3, 0]).double(), 2.0 ** -8 if dtype == "bf16" else 1e-6)
@@ -279,6 +282,25 @@ def test_student_that_has_learnt_the_list():
     x[1, ids[1].cpu()] = torch.randn(k, generator=g) + 5
     lp = torch.log_softmax(torch.randn(2, k, generator=g), -1) + math.log(0.999)
     check(x.cuda(), ids, lp.cuda())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,V,k", [(3, 3000, 9), (2, 40000, 100), (2700, 300, 5), (1, 33001, 3)])
+@pytest.mark.parametrize("gap", [40.0, 120.0, 400.0])
+def test_rest_far_below_the_list(R, V, k, gap):
+    """The list (and one of its ids twice) lies `gap` above all the rest, which exp(-gap) does not hold in
+    fp32 from 104 on: the rest's sum has a maximum of its own, so the loss (about the rest's share times the gap) and
+    the rest's gradients stay finite and right; a row whose list lies below the rest by as much, too."""
+    g = torch.Generator().manual_seed(int(gap) + V)
+    x = torch.randn(R, V, generator=g)
+    ids, lp = teacher(R, V, k, V, mass=0.8)
+    ids[0, 1] = ids[0, 0]
+    x.scatter_add_(1, ids.cpu(), torch.full((R, k), gap))
+    x[-1] = torch.randn(V, generator=g)
+    x[-1, ids[-1].cpu()] -= gap
+    for dtype in ("fp32", "bf16"):
+        check(x.to(TYPES[dtype]).cuda(), ids, lp)
+        check(x.to(TYPES[dtype]).cuda(), ids, lp, t=0.5)
 
 
 @pytest.mark.gpu
