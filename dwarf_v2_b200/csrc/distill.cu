@@ -1,26 +1,25 @@
 // Distillation from a teacher's top entries: per row KL(teacher || student) and
 // the gradient of the student's logits.
 //
-// With c = 1/temperature: over the ids that the teacher does not list, m_* = max x and
-// S_* = sum exp(c (x - m_*)); over the row, m and S likewise. The student's rest is
-// log q_* = c (m_* - m) + log S_* - log S, and
-//   loss = sum_k p_k (log p_k - c (x_k - m) + log S) + p_* (log p_* - log q_*)
+// With c = 1/temperature, m = max x, S = sum exp(c (x - m)) over the row, and S_* = sum exp(c
+// (x - m_*)) over the ids that the teacher does not list:
+//   loss = sum_k p_k (log p_k - c (x_k - m) + log S) + p_* (log p_* - c (m_* - m) - log S_* + log S)
 //   grad_v = s c (q_v W - [v listed] sum p - [v not listed] p_* exp(c (x_v - m_*)) / S_*),  W = sum p + p_*.
-// The rest has sums of its own, relative to a maximum of its own: S minus the listed
-// entries would cancel, and a sum relative to m would vanish, where the student has learnt
-// the list. A bit per vocabulary entry says what is listed; the listed entries' part of S
-// comes from their gathered logits.
+// S_* is a sum of its own: S minus the listed entries would cancel where the student has
+// learnt the list. A bit per vocabulary entry says what is listed. m_* is m; where the list lies so
+// far above the rest that S_* would vanish in fp32, the rest is summed once more relative to its own maximum.
 #include "vocab_row.cuh"
 
 namespace dwarf {
 namespace {
 
-// (m, sum relative to m) of a warp's lanes joined, in a fixed order; lanes without a part: m = -inf, sum 0.
-__device__ __forceinline__ void warp_join(float c2, float& m, float& sum) {
+// (m, sums relative to m) of a warp's lanes joined, in a fixed order; lanes without a part: m = -inf, sums 0.
+__device__ __forceinline__ void warp_join(float c2, float& m, float& a, float& b) {
   const float top = warp_max(m);
   const float f = ex2_approx((m - (top == -CUDART_INF_F ? 0.0f : top)) * c2);
   m = top;
-  sum = warp_sum(sum == 0.0f ? 0.0f : f * sum);
+  a = warp_sum(a == 0.0f ? 0.0f : f * a);
+  b = warp_sum(b == 0.0f ? 0.0f : f * b);
 }
 
 // One row, or a CTA's part of one. kKnown: the gradient from the sums that a launch with
@@ -32,10 +31,10 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
   constexpr int kSlots = NT < DWARF_TOP_K_MAX ? DWARF_TOP_K_MAX / NT : 1;  // slots of the teacher's list for a thread
   constexpr int kListWarps = NT < DWARF_TOP_K_MAX ? kWarps : DWARF_TOP_K_MAX / 32;
   extern __shared__ __align__(16) uint32_t listed[];  // a bit for each place of the part
-  __shared__ float s_m[kWarps], s_rest[kWarps];
-  __shared__ float s_top[kListWarps], s_term[kListWarps], s_list_m[kListWarps], s_list[kListWarps];
+  __shared__ float s_m[kWarps], s_rest[kWarps], s_list[kWarps];
+  __shared__ float s_top[kListWarps], s_term[kListWarps];
   __shared__ double s_sum[kListWarps];
-  __shared__ float s_parts[kMaxCluster][2];
+  __shared__ float s_parts[kMaxCluster][3], s_own[kMaxCluster][2];
   __shared__ int s_id[DWARF_TOP_K_MAX];
   __shared__ float s_p[DWARF_TOP_K_MAX];
   __shared__ int s_flags, s_listed;
@@ -120,97 +119,151 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
 
   const float c2 = a.inv_temperature * kLog2e;
   const float2 cc = make_float2(c2, c2);
-  float m_rest = -CUDART_INF_F, s_r, m, total, rest = 0.0f;
+  auto teacher_sum = [&] {
+    double sum_p = 0.0;
+#pragma unroll
+    for (int w = 0; w < kListWarps; ++w) sum_p += s_sum[w];
+    return sum_p;
+  };
+  float m = -CUDART_INF_F, m_rest, s_r, total, rest = 0.0f;
   if (!kKnown) {
-    // the listed entries' logits: maximum and sum, each id once
-    if (warp < kListWarps) {
-      float list_m = -CUDART_INF_F, list = 0.0f;
-      bool once[kSlots];
-#pragma unroll
-      for (int s = 0; s < kSlots; ++s) {
-        once[s] = id[s] >= 0 && id[s] < vocab;
-        if (once[s] && (cluster > 1 || (s_flags & 1)))  // a CTA of a cluster sees its own part's repetitions alone
-          for (int j = 0; j < tid + s * NT; ++j) once[s] &= s_id[j] != id[s];
-        if (once[s]) list_m = fmaxf(list_m, xv[s]);
-      }
-      list_m = warp_max(list_m);
-      const float base = list_m == -CUDART_INF_F ? 0.0f : list_m;
-#pragma unroll
-      for (int s = 0; s < kSlots; ++s)
-        if (once[s]) list += ex2_approx((xv[s] - base) * c2);
-      list = warp_sum(list);
-      if (lane == 0) s_list_m[warp] = list_m, s_list[warp] = list;
-    }
-    float2 sum = make_float2(0.0f, 0.0f);  // the ids not listed
+    float s_l;
+    float2 sum = make_float2(0.0f, 0.0f), sum_list = sum;
     for (int at = 0; at < part.size(); at += kTile) {
       uint4 v[kVectors];
       if (kTwice) part.load(at, v, keep); else part.load(at, v);
+      typename V::Max mv = V::max_of(v[0]);
+#pragma unroll
+      for (int i = 1; i < kVectors; ++i) mv = V::join(mv, V::max_of(v[i]));
+      const float m_new = fmaxf(m, warp_max(V::largest(mv)));
+      if (m > -CUDART_INF_F) {  // a later tile: move the sums to the new maximum
+        const float f = ex2_approx((m - m_new) * c2);
+        sum = mul2(sum, make_float2(f, f));
+        sum_list = mul2(sum_list, make_float2(f, f));
+      }
+      m = m_new;
+      const float s = m == -CUDART_INF_F ? 0.0f : -m;
       // the bits of a thread's vectors of a tile lie NT kVec / 8 bytes apart
       const int place = part.w0 - part.j0 + at + tid;
       const unsigned char* bits = reinterpret_cast<const unsigned char*>(listed) + place * V::kVec / 8;
       const int bits_shift = V::kVec == 4 ? 4 * (place & 1) : 0;
-      const bool whole = at + kTile <= part.size();
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i) {
-        if (!whole && at + i * NT + tid >= part.size()) break;  // vectors past the part hold -inf
-        const uint32_t mask = (bits[i * NT * V::kVec / 8] >> bits_shift) & ((1u << V::kVec) - 1u);
-        if (mask != 0) v[i] = V::drop(v[i], mask);
-      }
-      typename V::Max mv = V::max_of(v[0]);
-#pragma unroll
-      for (int i = 1; i < kVectors; ++i) mv = V::join(mv, V::max_of(v[i]));
-      const float m_new = fmaxf(m_rest, warp_max(V::largest(mv)));
-      if (m_rest > -CUDART_INF_F) {  // a later tile: move the sums to the new maximum
-        const float f = ex2_approx((m_rest - m_new) * c2);
-        sum = mul2(sum, make_float2(f, f));
-      }
-      m_rest = m_new;
-      const float s = m_rest == -CUDART_INF_F ? 0.0f : -m_rest;
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i) {
-        if (at + i * NT >= part.size()) break;
+      auto add = [&](const uint4& w, uint32_t mask) {
         float2 e[V::kVec / 2];
-        V::unpack(v[i], e);
+        V::unpack(w, e);
 #pragma unroll
         for (int h = 0; h < V::kVec / 2; ++h) {
           const float2 d = mul2(add2(e[h], make_float2(s, s)), cc);
-          sum = add2(sum, make_float2(ex2_approx(d.x), ex2_approx(d.y)));
+          e[h] = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+        }
+        if (mask != 0) {
+#pragma unroll
+          for (int h = 0; h < V::kVec / 2; ++h) {
+            if (mask & (1u << (2 * h))) sum_list.x += e[h].x, e[h].x = 0.0f;
+            if (mask & (2u << (2 * h))) sum_list.y += e[h].y, e[h].y = 0.0f;
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < V::kVec / 2; ++h) sum = add2(sum, e[h]);
+      };
+      if (at + kTile <= part.size()) {
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i)
+          add(v[i], (bits[i * NT * V::kVec / 8] >> bits_shift) & ((1u << V::kVec) - 1u));
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+          if (at + i * NT >= part.size()) break;
+          const bool in = at + i * NT + tid < part.size();  // vectors outside hold -inf
+          add(v[i], in ? (bits[i * NT * V::kVec / 8] >> bits_shift) & ((1u << V::kVec) - 1u) : 0u);
         }
       }
     }
     if (warp == 0 && part.ends()) {
-      const int at = end_id + part.row.lead - part.j0 * V::kVec;
-      const float own = end_id >= 0 && !((listed[at >> 5] >> (at & 31)) & 1u) ? end : -CUDART_INF_F;
-      const float m_new = fmaxf(m_rest, warp_max(own)), base = m_new == -CUDART_INF_F ? 0.0f : m_new;
-      const float f = ex2_approx((m_rest - base) * c2);
+      const float m_new = fmaxf(m, warp_max(end)), base = m_new == -CUDART_INF_F ? 0.0f : m_new;
+      const float f = ex2_approx((m - base) * c2), e = ex2_approx((end - base) * c2);
       sum = mul2(sum, make_float2(f, f));
-      sum.x += ex2_approx((own - base) * c2);
-      m_rest = m_new;
+      sum_list = mul2(sum_list, make_float2(f, f));
+      const int at = end_id + part.row.lead - part.j0 * V::kVec;
+      if (end_id >= 0 && ((listed[at >> 5] >> (at & 31)) & 1u)) sum_list.x += e; else sum.x += e;
+      m = m_new;
     }
     s_r = warp_sum(sum.x + sum.y);
-    if (lane == 0) s_m[warp] = m_rest, s_rest[warp] = s_r;
+    s_l = warp_sum(sum_list.x + sum_list.y);
+    if (lane == 0) s_m[warp] = m, s_rest[warp] = s_r, s_list[warp] = s_l;
     if (k >= vocab) {  // every id may be listed: nothing is left to be the rest
       for (int i = tid; i < words; i += NT) atomicAdd(&s_listed, __popc(listed[i]));
     }
     __syncthreads();
     // every warp joins the warps' sums, then the parts' sums, in the same order
     s_r = lane < kWarps ? s_rest[lane] : 0.0f;
-    m_rest = lane < kWarps ? s_m[lane] : -CUDART_INF_F;
-    warp_join(c2, m_rest, s_r);
+    s_l = lane < kWarps ? s_list[lane] : 0.0f;
+    m = lane < kWarps ? s_m[lane] : -CUDART_INF_F;
+    warp_join(c2, m, s_r, s_l);
     if (cluster > 1) {
-      if (tid < 2 * cluster) st_cluster(cluster_address(&s_parts[rank][tid & 1], tid >> 1), tid & 1 ? s_r : m_rest);
+      if (tid < 3 * cluster)
+        st_cluster(cluster_address(&s_parts[rank][tid % 3], tid / 3), tid % 3 == 0 ? m : tid % 3 == 1 ? s_r : s_l);
       cluster_arrive();
       cluster_wait();
-      m_rest = lane < cluster ? s_parts[lane][0] : -CUDART_INF_F;
+      m = lane < cluster ? s_parts[lane][0] : -CUDART_INF_F;
       s_r = lane < cluster ? s_parts[lane][1] : 0.0f;
-      warp_join(c2, m_rest, s_r);
+      s_l = lane < cluster ? s_parts[lane][2] : 0.0f;
+      warp_join(c2, m, s_r, s_l);
     }
-    // the row: the rest and the list
-    m = lane < kListWarps ? s_list_m[lane] : lane == 31 ? m_rest : -CUDART_INF_F;
-    total = lane < kListWarps ? s_list[lane] : lane == 31 ? s_r : 0.0f;
-    warp_join(c2, m, total);
     if (m == -CUDART_INF_F) m = 0.0f;
-    if (m_rest == -CUDART_INF_F) m_rest = 0.0f;
+    m_rest = m;
+    total = s_r + s_l;
+    if (a.tail && s_listed != vocab) {
+      const double sum_p = teacher_sum();
+      rest = sum_p == sum_p ? (float)fmax(0.0, 1.0 - sum_p) : CUDART_NAN_F;
+    }
+    // Entries below 2^-126 of the maximum count as 0. While the rest is 2^-40 or more, they are at
+    // most 2^-66 of it together, and the share of each in its gradient 2^-86. Below, the rest
+    // is summed again, relative to its own maximum.
+    if (rest > 0.0f && s_r < 0x1p-40f) {
+      m_rest = -CUDART_INF_F;
+      s_r = 0.0f;
+      for (int at = -NT; at < part.size(); at += NT) {  // the row's ends, then a vector a thread
+        uint4 v = make_uint4(V::kMinusInf, V::kMinusInf, V::kMinusInf, V::kMinusInf);
+        const int place = part.w0 - part.j0 + at + tid;
+        if (at >= 0 && at + tid < part.size()) {
+          v = part.row.load(part.w0 + at + tid);
+          const uint32_t bits = listed[place * V::kVec / 32] >> (place * V::kVec % 32);
+          v = V::drop(v, bits & ((1u << V::kVec) - 1u));
+        }
+        float own = V::largest(V::max_of(v));
+        const int end_at = end_id + part.row.lead - part.j0 * V::kVec;
+        if (at < 0 && end_id >= 0 && !((listed[end_at >> 5] >> (end_at & 31)) & 1u)) own = end;
+        const float m_new = fmaxf(m_rest, warp_max(own)), base = m_new == -CUDART_INF_F ? 0.0f : m_new;
+        s_r *= m_rest == -CUDART_INF_F ? 0.0f : ex2_approx((m_rest - base) * c2);
+        if (at < 0) {
+          s_r += ex2_approx((own - base) * c2);
+        } else {
+          float2 e[V::kVec / 2];
+          V::unpack(v, e);
+#pragma unroll
+          for (int h = 0; h < V::kVec / 2; ++h)
+            s_r += ex2_approx((e[h].x - base) * c2) + ex2_approx((e[h].y - base) * c2);
+        }
+        m_rest = m_new;
+      }
+      s_r = warp_sum(s_r);
+      __syncthreads();  // all have read the earlier sums
+      if (lane == 0) s_m[warp] = m_rest, s_rest[warp] = s_r;
+      __syncthreads();
+      float none = 0.0f;
+      s_r = lane < kWarps ? s_rest[lane] : 0.0f;
+      m_rest = lane < kWarps ? s_m[lane] : -CUDART_INF_F;
+      warp_join(c2, m_rest, s_r, none);
+      if (cluster > 1) {
+        if (tid < 2 * cluster) st_cluster(cluster_address(&s_own[rank][tid & 1], tid >> 1), tid & 1 ? s_r : m_rest);
+        cluster_arrive();
+        cluster_wait();
+        m_rest = lane < cluster ? s_own[lane][0] : -CUDART_INF_F;
+        s_r = lane < cluster ? s_own[lane][1] : 0.0f;
+        warp_join(c2, m_rest, s_r, none);
+      }
+      if (m_rest == -CUDART_INF_F) m_rest = 0.0f;
+    }
   } else {
     const float4* known = reinterpret_cast<const float4*>(a.stats) + 2 * r;
     const float4 first = known[0];
@@ -220,25 +273,17 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
   const bool off = s_flags & 2;
   float weight = 1.0f;
   if (a.tail) {
-    double sum_p = 0.0;
-#pragma unroll
-    for (int w = 0; w < kListWarps; ++w) sum_p += s_sum[w];
-    if (!kKnown) {
-      rest = s_listed == vocab ? 0.0f : (float)fmax(0.0, 1.0 - sum_p);
-      if (sum_p != sum_p) rest = CUDART_NAN_F;
-    }
-    weight = (float)(sum_p + (double)rest);
+    weight = (float)(teacher_sum() + (double)rest);
   } else {
-    float top = -CUDART_INF_F, sum_p = 0.0f;
+    float top = -CUDART_INF_F, all = 0.0f;
 #pragma unroll
     for (int w = 0; w < kListWarps; ++w) top = fmaxf(top, s_top[w]);
 #pragma unroll
-    for (int w = 0; w < kListWarps; ++w)
-      sum_p += s_sum[w] == 0.0 ? 0.0f : (float)s_sum[w] * expf(s_top[w] - top);
-    const float ln_sum = logf(sum_p);
+    for (int w = 0; w < kListWarps; ++w) all += s_sum[w] == 0.0 ? 0.0f : (float)s_sum[w] * expf(s_top[w] - top);
+    const float ln_sum = logf(all);
 #pragma unroll
     for (int s = 0; s < kSlots; ++s) l[s] = l[s] - top - ln_sum;
-    if (!(sum_p > 0.0f)) weight = CUDART_NAN_F;  // no slot with a finite value
+    if (!(all > 0.0f)) weight = CUDART_NAN_F;  // no slot with a finite value
   }
   if (off) weight = CUDART_NAN_F;
   float p[kSlots], term = 0.0f;

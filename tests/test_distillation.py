@@ -5,7 +5,8 @@ p (log p - log q): p is off by 2^-22 + |log p| 2^-23 relative, log p and log q b
 their size, so the loss by ``(4 rel + (k + 8) 2^-24)`` times the sum of the magnitudes of its terms, each taken
 with 1 + |log p| <= 24, plus rel for the logarithms themselves (sum p <= 1). p_* = 1 - sum p is off by 2^-22
 absolute, which its logarithm turns into 2^-22 (1 + |log p_* - log q_*|): p_* log p_* moves by that much.
-Gradients are held entry by entry to that share of the magnitudes of their terms plus one rounding (eps / 2).
+Gradients are held entry by entry to that share of the magnitudes of their terms plus one rounding (eps / 2);
+an entry below 2^-126 of the row's maximum may be left without its share of the rest, 2^-86 of it.
 """
 
 import math
@@ -30,7 +31,7 @@ def tolerances(x, ids, lp, t, loss_size, grad, size, tail):
     share = 4 * rel + (k + 32) * 2.0 ** -24
     loss_tol = torch.nan_to_num(loss_size) * share + 2 * rel + (2.0 ** -18 if tail else 0.0)
     d = torch.nan_to_num((x.double() - x.double().amax(-1, keepdim=True)) / t, neginf=0.0).abs()
-    tiny = 2.0 ** -24 if x.dtype == torch.float16 else 2.0 ** -120
+    tiny = 2.0 ** -24 if x.dtype == torch.float16 else 2.0 ** -86
     grad_tol = (torch.nan_to_num(size) * (2 * share + d * 2.0 ** -21)
                 + torch.finfo(x.dtype).eps / 2 * torch.nan_to_num(grad).abs() * 1.01 + tiny)
     return loss_tol, grad_tol
