@@ -357,16 +357,17 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
 // The loss, and with kGrad the gradient in the same launch: the row is then read twice, the
 // second time from L2. One bulk prefetch at the start fetches the row while the teacher's list
 // is read, under a policy that keeps it there, and the threads of a CTA are chosen so that the
-// rows in flight are about 40 MB. 16384 rows of 32768 bf16, 64 entries: 383 us (128 threads
+// rows in flight are about 40 MB. 16384 rows of 32768 bf16, 64 entries: 390 us (128 threads
 // without either: 534, with 475 MB read for 268; the row held in shared memory: 483; 512
-// threads: 540). The loss alone: 128 threads, no prefetch, 196 us (256 threads: 249).
+// threads: 540). The loss alone: 128 threads, no prefetch, 199 us (256 threads: 249).
 template <typename T, int NT, bool kGrad>
 __global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_kernel(const dwarf_topk_distill_args a, int cluster) {
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
   distill_row<T, NT, kGrad, false>(a, cluster, rank, blockIdx.x / (unsigned)cluster);
 }
 
-// The gradient from the sums of an earlier launch. With skip_if_one a grid of one wave, which
+// The gradient from the sums of an earlier launch: one read and one write (368 us at 16384
+// rows of 32768 bf16, 5.8 TB/s). With skip_if_one a grid of one wave, which
 // costs 3 us (a CTA for each of 16384 rows: 11 us) where there is nothing to do.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_grad_kernel(const dwarf_topk_distill_args a, int parts) {

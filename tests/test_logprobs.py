@@ -151,6 +151,30 @@ def test_row_addressing():
     assert addressed(torch.zeros(2, 0, 10))[1] * addressed(torch.zeros(2, 0, 10))[2] == 0
 
 
+def test_launches_on_the_tensors_device(monkeypatch):
+    """A launch goes to the current device: the tensors' one is made current for it, and only where it is not."""
+    from dwarf_v2_b200 import _lib, _rows
+
+    current, seen = [0], []
+
+    class Device:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(_lib, "call", lambda name, args, device: seen.append((name, current[0], device.index)))
+    for index in (0, 3):
+        _rows.launch("dwarf_row_reduce", None, torch.device("cuda", index))
+    assert seen == [("dwarf_row_reduce", 0, 0), ("dwarf_row_reduce", 3, 3)] and current == [0]
+
+
 def test_c_entry_refuses_bad_arguments():
     import ctypes
 
