@@ -87,6 +87,11 @@ def stream_handle(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def capture_id(device: torch.device) -> int:
+    """The id of the capture into a CUDA graph that runs on the device's current stream, 0 when none does."""
+    return load().dwarf_capture_id(stream_handle(device))
+
+
 def check(status: int, what: str) -> None:
     if status == 0:
         return
@@ -401,5 +406,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         fn = getattr(lib, name)
         fn.restype = c_i32
         fn.argtypes = [ctypes.POINTER(struct), c_ptr]
+    lib.dwarf_capture_id.restype = c_i64
+    lib.dwarf_capture_id.argtypes = [c_ptr]
     lib.dwarf_ema_scan_workspace_bytes.restype = c_i64
     lib.dwarf_ema_scan_workspace_bytes.argtypes = [c_i64, c_i64, c_i64, c_i32]

@@ -19,3 +19,13 @@ extern "C" const char* dwarf_status_string(int status) {
 }
 
 extern "C" int dwarf_abi_version(void) { return DWARF_ABI_VERSION; }
+
+extern "C" int64_t dwarf_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+    (void)cudaGetLastError();  // the legacy stream while another captures
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusActive ? (int64_t)id : 0;
+}

@@ -11,7 +11,9 @@ Where the loss is reduced (``"mean"``, ``"sum"``) and the logits require grad,
 the forward launch writes the gradient for an upstream gradient of 1 in the same
 pass over the logits; backward's launch leaves it as it is when the upstream
 gradient is 1, and otherwise computes it anew from the logits and the sums that the
-forward launch has left (one rounding either way). ``weight`` scales the loss without leaving the one-pass form.
+forward launch has left (one rounding either way). Where the two do not run alike (one
+captured into a CUDA graph and the other not) backward always computes it.
+``weight`` scales the loss without leaving the one-pass form.
 """
 
 from __future__ import annotations
@@ -56,6 +58,7 @@ class _TopKDistillationFn(torch.autograd.Function):
         ctx.grad = None
         if reduction != "none":
             ctx.grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            ctx.capture = _lib.capture_id(logits.device)
         loss, ctx.scale, ctx.grad_scale = _forward(logits, ids, logprobs, mask, inv_temperature, tail, reduction,
                                                    weight, ctx.grad, stats)
         return loss
@@ -66,7 +69,9 @@ class _TopKDistillationFn(torch.autograd.Function):
             return _once_more(ctx, g)
         logits, ids, logprobs, mask, stats = ctx.saved_tensors
         grad, ctx.grad = ctx.grad, None  # a second backward gets a buffer of its own
-        written = grad is not None
+        # Where only one of forward and backward is captured, or each into a graph of its own, they are not
+        # replayed in step, and what forward wrote is not this backward's to hand out.
+        written = grad is not None and ctx.capture == _lib.capture_id(logits.device)
         if not written:
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         _launch(logits, ids, logprobs, mask, *ctx.scalars, grad=grad, stats=stats, grad_scale=ctx.grad_scale,

@@ -59,6 +59,8 @@ typedef enum {
 const char* dwarf_status_string(int status);
 /* Returns DWARF_ABI_VERSION of the loaded library. */
 int dwarf_abi_version(void);
+/* The id of the capture (into a CUDA graph) that is under way on a stream, 0 when none is. */
+int64_t dwarf_capture_id(void* stream);
 
 /* ------------------------------------------------------------------------
  * Causal EMA scan.

@@ -385,6 +385,54 @@ def test_streams_and_graphs():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_one_direction_captured(reduction):
+    """A captured forward with eager backwards: a gradient handed out stays as it is through later replays. An eager
+    forward with a captured backward: each replay writes the gradient, whatever was done to the last one."""
+    from dwarf_v2_b200.distillation import topk_distillation_loss
+
+    x = logits(33, 4096, "bf16", 8).cuda()
+    moved = x.roll(3, 1)
+    ids, lp = teacher(33, 4096, 16, 2)
+    up = torch.ones(33 if reduction == "none" else (), device="cuda")
+
+    def forward(leaf):
+        return topk_distillation_loss(leaf, ids, lp, reduction=reduction)
+
+    def right(got, v):
+        f = 1 / 33 if reduction == "mean" else 1.0
+        _, want, size, loss_size = oracle.topk_distillation(v, ids, lp)
+        close(got, want * f, tolerances(v, ids, lp, 1.0, loss_size, want * f, size * f, True)[1])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        static = x.clone().requires_grad_()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            loss = forward(static)
+        graph.replay()
+        g1, = torch.autograd.grad(loss, static, up, retain_graph=True)
+        right(g1, x)
+        kept = g1.clone()
+        static.data.copy_(moved)
+        graph.replay()
+        g2, = torch.autograd.grad(loss, static, up, retain_graph=True)
+        right(g2, moved)
+        assert torch.equal(g1, kept)
+
+        leaf = x.clone().requires_grad_()
+        loss = forward(leaf)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            g3, = torch.autograd.grad(loss, leaf, up, retain_graph=True)  # replays read what forward saved
+        for _ in range(2):
+            g3.zero_()
+            graph.replay()
+            right(g3, x)
+
+
+@pytest.mark.gpu
 def test_teacher_to_student():
     """As used: a teacher's top alternatives at a temperature feed the student's loss; equal models give a
     divergence of zero and a gradient of zero, up to the roundings."""
