@@ -301,12 +301,14 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : kTop ? 9 : 8)
     float2 s = make_float2(0.0f, 0.0f), t = s;
     // Entries 2^-200 below the maximum count as 0, masked ones among them (0 (-inf) is
     // not formed). Where the row's type has room for such a bound below the maximum
-    // (2^-60 at least) and c m is no extreme value, the bound is set in packed pairs and
-    // d = c x - c m takes one fused operation; what the rounding of c m leaves out is put
-    // back into the sums. Otherwise d = c (x - m) and the bound is set in fp32.
+    // (2^-60 at least) and |c m| is below 2^20, the bound is set in packed pairs and
+    // d = c x - c m takes one fused operation; what the rounding of c m leaves out (2^-5 at
+    // most) is put back into the sums. Otherwise d = c (x - m) and the bound is set in fp32:
+    // from |c m| = 2^31 on the part left out can pass an exponent's range (fp32 logits of 16 at
+    // temperature 1e-8), and with it every sum of the row.
     const typename V::Low low = V::low_of(m - 200.0f / c2);
     const float cm = m * c2;
-    if ((m - V::low_value(low)) * c2 >= 60.0f && V::low_value(low) > -1.0e38f && fabsf(cm) < 1.0e30f) {
+    if ((m - V::low_value(low)) * c2 >= 60.0f && V::low_value(low) > -1.0e38f && fabsf(cm) < 0x1p20f) {
       const float2 shift = make_float2(-cm, -cm), cc = make_float2(c2, c2);
       auto add = [&](const uint4& w) {
         float2 e[V::kVec / 2];

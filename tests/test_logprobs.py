@@ -530,3 +530,60 @@ def test_rows_past_32_bit_offsets():
     want, size = oracle.token_logprobs_grad(tail, targets[-3:], g_logprob=up[-3:])
     close(grad[-3:], want, grad_tolerance(tail, 1.0, want, size))
     assert not bool((grad[:-3] != 0).any())
+
+
+# ------------------------------------------------------------------ scaled maxima past the range of the packed form
+
+
+def _near_ties(R, V, seed, low, high):
+    """fp32 rows whose maxima are spread over [low, high], and whose best entries lie a few steps of the type apart:
+    a step times 1 / temperature is from far below to far above 1."""
+    g = torch.Generator().manual_seed(seed)
+    top = low * (high / low) ** torch.rand(R, 1, generator=g)
+    x = top * torch.rand(R, V, generator=g)
+    at = torch.stack([torch.randperm(V, generator=g)[:12] for _ in range(R)])
+    steps = torch.randint(0, 6, (R, 12), generator=g).float()
+    steps[:, 0] = 0
+    best = (top.view(torch.int32) - steps.int()).view(torch.float32)
+    return x.scatter_(1, at, best), at[:, 3]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1e-12, 1e-10, 1e-9, 5e-9, 1e-8, 2e-8, 3e-8, 1e-7, 1e-6, 1e-5])
+@pytest.mark.parametrize("R,V", [(2000, 300), (3000, 261), (6, 20000)])  # 128 threads, a warp for each row, clusters
+def test_small_temperatures(R, V, t):
+    """c m of up to 10^14: a float's step there is far above the range of an exponent, and d = c x - c m formed from
+    the rounded c m would be as far off. The tolerances are those of every temperature: x - m is exact between
+    neighbours, so d has its three roundings."""
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    x, targets = _near_ties(R, V, int(-math.log10(t) * 100) + V, 1.0, 130.0)
+    x, targets = x.cuda(), targets.cuda()
+    check_forward(token_logprobs(x, targets, temperature=t), x, targets, 0, t)
+    leaf = x.clone().requires_grad_()
+    out = token_logprobs(leaf, targets, top_k=4, temperature=t)
+    check_forward(out, x, targets, 4, t)
+    g = torch.Generator().manual_seed(3)
+    gl, gh = torch.randn(R, generator=g).cuda() * t, torch.randn(R, generator=g).cuda() * t  # c g is of the order of 1
+    gt = torch.randn(R, 4, generator=g).cuda() * t
+    grad, = torch.autograd.grad([out.logprob, out.entropy, out.top_logprobs], leaf, [gl, gh, gt])
+    want, size = oracle.token_logprobs_grad(x, targets, top_ids=out.top_ids, g_logprob=gl, g_entropy=gh, g_top=gt,
+                                            temperature=t)
+    # (c g is up to 5, and five such terms: the share of an exponential that counts as 0 is below 2^-119 still, by
+    # 2^-126 (5 + 5 + 5 (88 + 6)) < 2^-117 at most)
+    close(grad, want, grad_tolerance(x, t, want, size) + 2.0 ** -117, "grad")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [3e7, 3e9, -3e9, 1e20])
+@pytest.mark.parametrize("R,V", [(2000, 300), (3000, 261)])
+def test_far_offsets(R, V, offset):
+    """The same scaled maxima at temperature 1, from logits that lie far from 0 (steps of 2, 256 and more)."""
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    x, targets = _near_ties(R, V, 5, abs(offset), 1.3 * abs(offset))
+    if offset < 0:
+        x = x + 2 * offset
+    x, targets = x.cuda(), targets.cuda()
+    for t in (1.0, 150.0):
+        check_forward(token_logprobs(x, targets, top_k=3, temperature=t), x, targets, 3, t)
