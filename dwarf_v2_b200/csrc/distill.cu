@@ -262,7 +262,7 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
         s_r = lane < cluster ? s_own[lane][1] : 0.0f;
         warp_join(c2, m_rest, s_r, none);
       }
-      if (m_rest == -CUDART_INF_F) m_rest = 0.0f;
+      if (m_rest == -CUDART_INF_F) m_rest = m;  // nothing: the loss is inf, the entries' gradients 0
     }
   } else {
     const float4* known = reinterpret_cast<const float4*>(a.stats) + 2 * r;

@@ -128,6 +128,9 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teac
     * ``row_mask`` [...] bool: rows where it is False, and rows without a used slot,
       have loss 0 and gradient exactly 0 whatever their logits hold. A NaN or +inf among
       another row's logits makes its loss and gradient NaN.
+    * Where the student gives a listed id, or all the ids not listed, nothing (-inf) and the
+      teacher gives them something, the loss is inf and the gradient finite: -p / temperature
+      at such a listed id, 0 at the ids not listed.
     * ``reduction``: "mean" over the rows that ``row_mask`` keeps, "sum", or "none"
       ([...]). The loss is fp32; no factor temperature**2 is applied.
 

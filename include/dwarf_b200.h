@@ -812,7 +812,9 @@ int dwarf_token_logprobs_bwd(const dwarf_token_logprobs_bwd_args* args, void* st
  * (p_* = 0 when every id is listed). Slots with an id below 0 are not used; an
  * id >= vocab makes its row NaN; an id listed twice counts with both p. Rows
  * with row_mask 0 or without a used slot: loss and gradient exact zeros, the
- * logits not used. A NaN or +inf among another row's logits makes it NaN.
+ * logits not used. A NaN or +inf among another row's logits makes it NaN. A
+ * row whose ids not listed are all at -inf while the teacher leaves them a
+ * rest: loss +inf, their gradient 0 (the others' as below).
  *   grad_v = s c (q_v (sum p + p_*) - sum over slots with id v of p - [v not listed] p_* q_v / q_*)
  * where s = scale * (grad_scale ? *grad_scale : 1) * (grad_rows ? grad_rows[row or 0] : 1).
  * A launch for the gradient alone reads the row once, with the sums that the

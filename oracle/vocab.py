@@ -125,7 +125,9 @@ def topk_distillation(x, ids, logprobs, *, temperature=1.0, tail=True, row_mask=
                  + rest_term.abs().squeeze(-1) + rest.squeeze(-1) * logq_rest.clamp(min=-1e4).abs().squeeze(-1))
     q = torch.exp(logq)
     mass = torch.zeros_like(x).scatter_add_(-1, at, torch.where(used, p, zero))
-    share = torch.where(hit | (rest == 0), torch.zeros_like(x), rest * torch.exp(logq - logq_rest))
+    # (where the student gives the ids not listed nothing, the loss is inf and their gradient 0)
+    share = torch.where(hit | (rest == 0) | (logq_rest == -math.inf), torch.zeros_like(x),
+                        rest * torch.exp(logq - logq_rest))
     weight = p.sum(-1, keepdim=True) + rest
     grad, size = q * weight - mass - share, q * weight + mass + share
     up = torch.ones(R, dtype=torch.float64, device=x.device) if upstream is None else upstream.double()

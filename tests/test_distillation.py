@@ -452,3 +452,30 @@ def test_teacher_to_student():
     close(got, grad, grad_tol)
     same = topk_distillation_loss(t_logits, top.top_ids, top.top_logprobs, temperature=2.0, reduction="none")
     assert same.abs().max() < 2.0 ** -16
+
+
+# ------------------------------------------------------------------ rows whose masks leave nothing to a part of the teacher
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("R,V,k", [(3, 300, 6), (2, 40000, 20), (1, 33001, 3), (2700, 261, 5)])
+@pytest.mark.parametrize("shift", [-2000.0, -200.0, 0.0, 200.0])
+def test_nothing_outside_the_list(R, V, k, shift, dtype):
+    """Every logit outside the list is -inf and the teacher leaves a rest: the loss is inf; the listed entries have
+    their gradient and the others exact zeros, wherever the listed values lie."""
+    from dwarf_v2_b200.distillation import topk_distillation_loss
+
+    ids, lp = teacher(R, V, k, V + k)
+    g = torch.Generator().manual_seed(k)
+    x = torch.full((R, V), -math.inf).scatter_(1, ids.cpu(), torch.randn(R, k, generator=g) + shift)
+    x = x.to(TYPES[dtype]).cuda()
+    check(x, ids, lp)
+    leaf = x.clone().requires_grad_()
+    rows = topk_distillation_loss(leaf, ids, lp, reduction="none")
+    assert (rows == math.inf).all()
+    for loss in (rows.sum(), topk_distillation_loss(leaf, ids, lp, reduction="sum")):
+        for up in (1.0, 0.25):
+            grad, = torch.autograd.grad(loss, leaf, torch.tensor(up).cuda(), retain_graph=True)
+            assert torch.isfinite(grad).all()
+            assert not grad.scatter(1, ids, 0.0).any()
