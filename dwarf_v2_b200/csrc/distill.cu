@@ -287,7 +287,10 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
   }
   if (off) weight = CUDART_NAN_F;
   float p[kSlots], term = 0.0f;
-  const float ln_total = log2f(total) * kLn2;
+  // A row without a finite logit (m = 0 here): log q is -inf everywhere, so the loss is inf where
+  // the teacher gives anything, and the gradient 0 (NaN for a NaN teacher).
+  const bool empty = total == 0.0f;
+  const float ln_total = empty ? 0.0f : log2f(total) * kLn2;
 #pragma unroll
   for (int s = 0; s < kSlots; ++s) {
     p[s] = id[s] >= 0 ? expf(l[s]) : 0.0f;
@@ -303,7 +306,8 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
     sc = a.scale * a.inv_temperature;
     if (a.grad_scale != nullptr) sc *= *a.grad_scale;
     if (a.grad_rows != nullptr) sc *= a.grad_rows[a.grad_rows_stride ? r : 0];
-    k_list = sc * weight / total;
+    k_list = empty ? 0.0f * weight : sc * weight / total;
+    if (empty) sc = 0.0f;
     // of exp(c (x - m_*)): q_v W and the rest's share
     float k_rest = ex2_approx((m_rest - m) * c2) * k_list;
     if (rest > 0.0f && s_r > 0.0f) k_rest -= sc * rest / s_r;

@@ -130,7 +130,8 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teac
       another row's logits makes its loss and gradient NaN.
     * Where the student gives a listed id, or all the ids not listed, nothing (-inf) and the
       teacher gives them something, the loss is inf and the gradient finite: -p / temperature
-      at such a listed id, 0 at the ids not listed.
+      at such a listed id, 0 at the ids not listed. A counted row without a finite logit has
+      loss inf and gradient 0.
     * ``reduction``: "mean" over the rows that ``row_mask`` keeps, "sum", or "none"
       ([...]). The loss is fp32; no factor temperature**2 is applied.
 

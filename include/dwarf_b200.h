@@ -814,7 +814,8 @@ int dwarf_token_logprobs_bwd(const dwarf_token_logprobs_bwd_args* args, void* st
  * with row_mask 0 or without a used slot: loss and gradient exact zeros, the
  * logits not used. A NaN or +inf among another row's logits makes it NaN. A
  * row whose ids not listed are all at -inf while the teacher leaves them a
- * rest: loss +inf, their gradient 0 (the others' as below).
+ * rest: loss +inf, their gradient 0 (the others' as below). A row without a
+ * finite logit: loss +inf, gradient 0 (0 and 0 where the teacher gives nothing).
  *   grad_v = s c (q_v (sum p + p_*) - sum over slots with id v of p - [v not listed] p_* q_v / q_*)
  * where s = scale * (grad_scale ? *grad_scale : 1) * (grad_rows ? grad_rows[row or 0] : 1).
  * A launch for the gradient alone reads the row once, with the sums that the

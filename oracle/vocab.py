@@ -102,7 +102,8 @@ def topk_distillation(x, ids, logprobs, *, temperature=1.0, tail=True, row_mask=
     if row_mask is not None:
         keep = keep & row_mask
     off = (ids >= V).any(-1) & keep
-    x = torch.where(keep.unsqueeze(-1), x, torch.zeros_like(x))
+    empty = (x == -math.inf).all(-1) & keep
+    x = torch.where((keep & ~empty).unsqueeze(-1), x, torch.zeros_like(x))
     at = ids.clamp(0, V - 1)
     l = torch.where(used, logprobs.double(), torch.full_like(logprobs, -math.inf, dtype=torch.float64))
     if tail:
@@ -134,7 +135,12 @@ def topk_distillation(x, ids, logprobs, *, temperature=1.0, tail=True, row_mask=
     up = up.unsqueeze(-1) / temperature
     dead = ~keep.unsqueeze(-1)
     grad = torch.where(dead, torch.zeros_like(grad), grad * up)
-    grad = torch.where(off.unsqueeze(-1), torch.full_like(grad, math.nan), grad)
+    # without a finite logit every q is 0, as its logarithm in token_logprobs says: the loss is inf, the gradient 0
+    given = weight.squeeze(-1)
+    nothing = torch.where(given > 0, torch.full_like(given, math.inf), given)
+    grad = torch.where(empty.unsqueeze(-1), torch.zeros_like(grad) * weight, grad)
+    loss = torch.where(empty, nothing, loss)
     loss = torch.where(keep, loss, torch.zeros_like(loss))
+    grad = torch.where(off.unsqueeze(-1), torch.full_like(grad, math.nan), grad)
     loss = torch.where(off, torch.full_like(loss, math.nan), loss)
     return loss, grad, size * up.abs(), loss_size

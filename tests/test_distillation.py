@@ -479,3 +479,46 @@ def test_nothing_outside_the_list(R, V, k, shift, dtype):
             grad, = torch.autograd.grad(loss, leaf, torch.tensor(up).cuda(), retain_graph=True)
             assert torch.isfinite(grad).all()
             assert not grad.scatter(1, ids, 0.0).any()
+
+
+def test_oracle_row_without_a_finite_logit():
+    x = torch.full((4, 6), -math.inf)
+    x[3] = 0.0
+    ids = torch.tensor([[1, 3], [1, -1], [-1, -1], [0, 1]])
+    lp = torch.log(torch.tensor([[0.5, 0.2], [0.9, 0.1], [0.3, 0.3], [0.5, 0.25]]))
+    for tail in (True, False):
+        loss, grad, size, _ = oracle.topk_distillation(x, ids, lp, tail=tail)
+        assert loss[:3].tolist() == [math.inf, math.inf, 0.0] and 0 < loss[3] < math.log(6)  # against an even q
+        assert not grad[:3].any() and grad[3].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("tail", [True, False])
+@pytest.mark.parametrize("R,V,k", [(5, 7, 2), (5, 1000, 6), (5, 40000, 20), (2700, 261, 5), (5, 4, 4)])
+def test_rows_without_a_finite_logit(R, V, k, tail, dtype):
+    """A counted row whose mask leaves nothing: loss inf, gradient 0; its neighbours are what they are without it,
+    and so is the gradient of a reduced loss. An id past the vocabulary or a NaN of the teacher still makes it NaN."""
+    from dwarf_v2_b200.distillation import topk_distillation_loss
+
+    ids, lp = teacher(R, V, k, V + k, mass=1.0 if k == V else 0.9)
+    x = logits(R, V, dtype, V)
+    x[1:-1] = -math.inf
+    x = x.cuda()
+    ids[2, 1:] = -1
+    if R > 4:
+        ids[3, 0] = V
+        lp[R - 2, 1] = math.nan
+    check(x, ids, lp, tail=tail, upstream=torch.linspace(0.5, 2.0, R).cuda())
+    mask = torch.ones(R, dtype=torch.bool).cuda()
+    mask[1:3] = False
+    check(x, ids, lp, tail=tail, row_mask=mask)
+    leaf = x.clone().requires_grad_()
+    good = [0, 1, 2, R - 1]
+    loss = topk_distillation_loss(leaf, ids, lp, tail=tail, reduction="none")
+    assert (loss[1:3] == math.inf).all() and torch.isfinite(loss[[0, R - 1]]).all()
+    assert torch.isnan(loss[3]) and torch.isnan(loss[R - 2])
+    grad, = torch.autograd.grad(topk_distillation_loss(leaf, ids, lp, tail=tail, reduction="sum"), leaf)
+    assert torch.isfinite(grad[good]).all() and not grad[1:3].any()
+    if k < V:  # (with every id listed and learnt there may be nothing to learn)
+        assert grad[0].any() and grad[R - 1].any()
