@@ -779,7 +779,7 @@ int dwarf_token_logprobs(const dwarf_token_logprobs_args* args, void* stream);
  *   grad_v = c (sum over entries with id v of their g - q_v (G + g_entropy (log q_v + entropy)))
  * A row whose gradients are all zero, or without a finite logit, gets exact
  * zeros and its logits are not used; a row whose target is neither
- * ignore_index nor in [0, vocab) gets NaN when g_logprob is given. */
+ * ignore_index nor in [0, vocab) gets NaN where its g_logprob is not 0. */
 typedef struct {
   int32_t version;
   int32_t dtype;                  /* of logits and grad                    */

@@ -587,3 +587,19 @@ def test_far_offsets(R, V, offset):
     x, targets = x.cuda(), targets.cuda()
     for t in (1.0, 150.0):
         check_forward(token_logprobs(x, targets, top_k=3, temperature=t), x, targets, 3, t)
+
+
+@pytest.mark.gpu
+def test_gradient_with_targets_outside():
+    """A target outside [0, V) makes its row's gradient NaN exactly where its log probability's gradient is not 0."""
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    x = logits(4, 300, "fp32", 2).cuda()
+    targets = torch.tensor([300, -1, 5, -100]).cuda()
+    leaf = x.clone().requires_grad_()
+    out = token_logprobs(leaf, targets)
+    gl, gh = torch.tensor([0.5, 0.0, 0.0, 1.0]).cuda(), torch.ones(4).cuda()
+    grad, = torch.autograd.grad([out.logprob, out.entropy], leaf, [gl, gh])
+    assert torch.isnan(grad[0]).all()
+    want, size = oracle.token_logprobs_grad(x[1:], g_entropy=gh[1:])
+    close(grad[1:], want, grad_tolerance(x[1:], 1.0, want, size))
