@@ -479,6 +479,12 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : kTop ? 9 : 8)
   }
 }
 
+// Bytes of the cells of a part of `vectors` vectors.
+constexpr int cell_bytes(int vectors, int threads) {
+  return (vectors + kVectors * threads - 1) / (kVectors * threads) * kCells * threads * 2;
+}
+constexpr int kMostVectors = 65536;  // of a part (cells: 64 KB)
+
 template <typename T, int NT>
 int launch_forward(const dwarf_token_logprobs_args& a, int64_t rows, int vectors, int cluster, cudaStream_t stream) {
   const int64_t wave = cluster > 1 ? rows : (NT == 32 ? 32 : a.top_k > 0 ? 9 : 8) * kNumSMs;  // rows in flight
@@ -487,12 +493,15 @@ int launch_forward(const dwarf_token_logprobs_args& a, int64_t rows, int vectors
     return launch_rows(kernel, rows, cluster, NT, 0, stream, a, cluster, 0, wave);
   }
   // a row that starts off a 16-byte boundary has one vector more
-  const int lists_at = ceil_div(ceil_div(vectors + 1, cluster), kVectors * NT) * kCells * NT * 2;
+  const int lists_at = cell_bytes(ceil_div(vectors + 1, cluster), NT);
   const int bytes = lists_at + (cluster > 1 ? cluster * a.top_k * 8 : 0);
   auto kernel = token_logprobs_kernel<T, NT, true, false>;
   if (NT != 32 && rows <= 4 * wave) kernel = token_logprobs_kernel<T, NT, true, NT != 32>;
+  // The limit is the kernel's, for all host threads: always the most that a call can need, so that
+  // a call with less cannot lower it before another one's launch.
+  constexpr int kMostBytes = cell_bytes(kMostVectors + 1, NT) + kMaxCluster * DWARF_TOP_K_MAX * 8;
   if (bytes > 32 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBytes) != cudaSuccess)
     return launch_status();
   return launch_rows(kernel, rows, cluster, NT, bytes, stream, a, cluster, lists_at, wave);
 }
@@ -503,7 +512,7 @@ int launch_forward(const dwarf_token_logprobs_args& a, cudaStream_t stream) {
   const int vectors = ceil_div((int)a.vocab, Vec16<T>::kVec);
   // (a warp's 64 groups bound up to 32 alternatives)
   if (a.top_k <= 32 && warp_rows(rows, vectors, 2048)) return launch_forward<T, 32>(a, rows, vectors, 1, stream);
-  return launch_forward<T, 128>(a, rows, vectors, cluster_for(rows, vectors, 65536), stream);  // cells: at most 64 KB
+  return launch_forward<T, 128>(a, rows, vectors, cluster_for(rows, vectors, kMostVectors), stream);
 }
 
 // grad_v = c (sparse terms - q_v (G + gH (log q_v + H))): each CTA writes its part of the

@@ -603,3 +603,38 @@ def test_gradient_with_targets_outside():
     assert torch.isnan(grad[0]).all()
     want, size = oracle.token_logprobs_grad(x[1:], g_entropy=gh[1:])
     close(grad[1:], want, grad_tolerance(x[1:], 1.0, want, size))
+
+
+@pytest.mark.gpu
+def test_host_threads_with_different_vocabularies():
+    """Rows whose alternatives take more than 32 KB of shared memory, of different sizes, from several threads at
+    once: the limit that one thread sets for the kernel must hold for another's launch."""
+    import ctypes
+    import threading
+
+    from dwarf_v2_b200 import _lib
+
+    lib, x, failed = _lib.load(), torch.zeros(1, 1 << 20, device="cuda"), []
+
+    def work(rows, vocab, calls):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            f, top = torch.zeros(rows, 2, device="cuda"), torch.zeros(rows, device="cuda")
+            ids = torch.zeros(rows, dtype=torch.int64, device="cuda")
+            args = _lib.TokenLogprobsArgs(version=_lib.ABI_VERSION, dtype=_lib.dtype_code(x.dtype), logits=x.data_ptr(),
+                                          outer=1, inner=rows, vocab=vocab, so=0, si=0, inv_temperature=1.0, top_k=1,
+                                          entropy=f.data_ptr(), lse=f.data_ptr() + 4 * rows,
+                                          top_logprobs=top.data_ptr(), top_ids=ids.data_ptr())
+            stream = torch.cuda.current_stream()
+            status = {lib.dwarf_token_logprobs(ctypes.byref(args), stream.cuda_stream) for _ in range(calls)}
+            stream.synchronize()
+            if status != {0} or ids.any():
+                failed.append((vocab, status))
+
+    torch.cuda.synchronize()
+    # one row: parts of 1 / 8; 80 rows: of 1 / 4
+    threads = [threading.Thread(target=work, args=a) for a in ((80, 1 << 20, 1500), (1, 1 << 20, 6000), (1, 1 << 20, 6000))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
