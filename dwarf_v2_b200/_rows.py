@@ -5,6 +5,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -27,6 +28,20 @@ def check_logits(logits: torch.Tensor, temperature: float) -> float:
     if not (math.isfinite(temperature) and 1e-30 <= temperature <= 1e30):
         raise ValueError(f"temperature must be positive and finite (1e-30..1e30), got {temperature}")
     return 1.0 / temperature
+
+
+def refuse_transforms(**tensors: torch.Tensor | None) -> None:
+    """Forward-mode derivatives and torch.func transforms are refused: a kernel reads a tensor's memory, where
+    a tangent or a batch dimension would be left out unseen."""
+    if forward_ad._current_level < 0 and torch._C._functorch.peek_interpreter_stack() is None:
+        return  # neither is under way
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if torch._C._functorch.is_functorch_wrapped_tensor(t):
+            raise NotImplementedError(f"{name}: torch.func transforms (vmap, grad, jvp, ...) are not supported")
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name}: forward-mode derivatives are not supported")
 
 
 def same_device(logits: torch.Tensor, **others: torch.Tensor | None) -> None:

@@ -135,10 +135,13 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teac
     * ``reduction``: "mean" over the rows that ``row_mask`` keeps, "sum", or "none"
       ([...]). The loss is fp32; no factor temperature**2 is applied.
 
-    Runs on the current stream, without synchronising.
+    Second and forward-mode derivatives and torch.func transforms are refused. Runs on the
+    current stream, without synchronising.
     """
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    _rows.refuse_transforms(logits=logits, teacher_ids=teacher_ids, teacher_logprobs=teacher_logprobs,
+                            row_mask=row_mask)
     inv_temperature = _rows.check_logits(logits, temperature)
     weight = float(weight)
     if not math.isfinite(weight):

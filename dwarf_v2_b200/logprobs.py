@@ -108,8 +108,10 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     A row without a finite logit gives logprob, lse and top_logprobs -inf, entropy 0
     and a gradient of zeros; a row with NaN or +inf gives NaN. Every float output is
     differentiable with respect to the logits; a row whose output gradients are all
-    zero gets exact zeros. Runs on the current stream, without synchronising.
+    zero gets exact zeros. Second and forward-mode derivatives and torch.func transforms
+    are refused. Runs on the current stream, without synchronising.
     """
+    _rows.refuse_transforms(logits=logits, targets=targets)
     inv_temperature = _rows.check_logits(logits, temperature)
     top_k = int(top_k)
     if not 0 <= top_k <= min(_rows.TOP_K_MAX, logits.shape[-1]):

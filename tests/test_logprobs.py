@@ -638,3 +638,33 @@ def test_host_threads_with_different_vocabularies():
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+def test_forward_mode_and_transforms_are_refused():
+    """A tangent or a batch dimension is refused before the tensors are looked at, not dropped."""
+    from torch.autograd import forward_ad
+
+    from dwarf_v2_b200.distillation import topk_distillation_loss
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    x, ids, lp = torch.randn(4, 10), torch.zeros(4, 3, dtype=torch.int64), torch.zeros(4, 3)
+    losses = (lambda v: topk_distillation_loss(v, ids, lp), lambda v: topk_distillation_loss(x, ids, v[:, :3]))
+    scores = (lambda v: token_logprobs(v).lse, lambda v: token_logprobs(v, ids[:, 0], top_k=2).logprob)
+    with forward_ad.dual_level():
+        for f in losses + scores:
+            for leaf in (x, x.clone().requires_grad_()):
+                with pytest.raises(NotImplementedError):
+                    f(forward_ad.make_dual(leaf, torch.ones_like(x)))
+            with torch.no_grad(), pytest.raises(NotImplementedError):  # no_grad does not stop a forward mode
+                f(forward_ad.make_dual(x, torch.ones_like(x))[:, :5])
+        with pytest.raises(RuntimeError, match="CUDA"):  # no tangent: as ever
+            token_logprobs(x)
+    for f in losses + scores:
+        for transform in (lambda f: torch.func.vmap(f)(x.expand(2, 4, 10)), lambda f: torch.func.jvp(f, (x,), (x,)),
+                          lambda f: torch.func.grad(lambda v: f(v).sum())(x),
+                          lambda f: torch.func.functionalize(f)(x)):
+            with pytest.raises(NotImplementedError):
+                transform(f)
+    for f in (lambda i: token_logprobs(x, i).logprob, lambda i: topk_distillation_loss(x, i[:, None], lp[:, :1])):
+        with pytest.raises(NotImplementedError):
+            torch.func.vmap(f)(ids[:, 0].expand(2, 4))
