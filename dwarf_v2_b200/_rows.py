@@ -44,6 +44,11 @@ def refuse_transforms(**tensors: torch.Tensor | None) -> None:
             raise NotImplementedError(f"{name}: forward-mode derivatives are not supported")
 
 
+def in_memory(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with its sign applied: a lazily negated view (the imaginary part of a conjugate) is copied."""
+    return t.resolve_neg() if t.is_neg() else t
+
+
 def same_device(logits: torch.Tensor, **others: torch.Tensor | None) -> None:
     """Every tensor on the logits' CUDA device."""
     _lib.require_cuda(logits, *others.values())

@@ -75,7 +75,7 @@ class _TopKDistillationFn(torch.autograd.Function):
         if not written:
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         _launch(logits, ids, logprobs, mask, *ctx.scalars, grad=grad, stats=stats, grad_scale=ctx.grad_scale,
-                grad_rows=g.contiguous(), skip_if_one=written, scale=ctx.scale)
+                grad_rows=_rows.in_memory(g).contiguous(), skip_if_one=written, scale=ctx.scale)
         return grad, None, None, None, None, None, None, None
 
 
@@ -142,6 +142,7 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teac
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
     _rows.refuse_transforms(logits=logits, teacher_ids=teacher_ids, teacher_logprobs=teacher_logprobs,
                             row_mask=row_mask)
+    logits = _rows.in_memory(logits)
     inv_temperature = _rows.check_logits(logits, temperature)
     weight = float(weight)
     if not math.isfinite(weight):
@@ -165,7 +166,7 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teac
             raise ValueError(f"row_mask must be {shape[:-1]}, got {tuple(row_mask.shape)}")
         row_mask = row_mask.contiguous()
     _rows.same_device(logits, teacher_ids=teacher_ids, teacher_logprobs=teacher_logprobs, row_mask=row_mask)
-    teacher_logprobs = teacher_logprobs.to(torch.float32).contiguous()
+    teacher_logprobs = _rows.in_memory(teacher_logprobs).to(torch.float32).contiguous()
     if grad and logits.requires_grad:
         return _TopKDistillationFn.apply(logits, teacher_ids, teacher_logprobs, row_mask, inv_temperature, bool(tail),
                                          reduction, weight)

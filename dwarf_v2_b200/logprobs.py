@@ -76,7 +76,7 @@ class _TokenLogprobsFn(torch.autograd.Function):
         top_k, inv_temperature, ignore_index = ctx.scalars
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         logits, outer, inner, so, si = _rows.addressed(logits)
-        g_logprob, g_entropy, g_lse, g_top = (None if g is None else g.contiguous()
+        g_logprob, g_entropy, g_lse, g_top = (None if g is None else _rows.in_memory(g).contiguous()
                                               for g in (g_logprob, g_entropy, g_lse, g_top))
         args = _lib.TokenLogprobsBwdArgs(
             version=_lib.ABI_VERSION, dtype=_lib.dtype_code(logits.dtype), logits=logits.data_ptr(), outer=outer,
@@ -112,6 +112,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     are refused. Runs on the current stream, without synchronising.
     """
     _rows.refuse_transforms(logits=logits, targets=targets)
+    logits = _rows.in_memory(logits)
     inv_temperature = _rows.check_logits(logits, temperature)
     top_k = int(top_k)
     if not 0 <= top_k <= min(_rows.TOP_K_MAX, logits.shape[-1]):

@@ -668,3 +668,38 @@ def test_forward_mode_and_transforms_are_refused():
     for f in (lambda i: token_logprobs(x, i).logprob, lambda i: topk_distillation_loss(x, i[:, None], lp[:, :1])):
         with pytest.raises(NotImplementedError):
             torch.func.vmap(f)(ids[:, 0].expand(2, 4))
+
+
+@pytest.mark.gpu
+def test_lazily_negated_views():
+    """Tensors whose sign is still to be applied (the imaginary part of a conjugate): logits, teacher, gradients."""
+    from dwarf_v2_b200.distillation import topk_distillation_loss
+    from dwarf_v2_b200.logprobs import token_logprobs
+
+    def negated(t):
+        z = torch.stack([torch.zeros_like(t), -t], -1)
+        view = torch.view_as_complex(z).conj().imag
+        assert view.is_neg() and torch.equal(view, t)
+        return view, torch._neg_view(-t)  # strided, contiguous
+
+    x = logits(5, 300, "fp32", 9).cuda()
+    ids, lp = torch.arange(4).repeat(5, 1).cuda(), torch.full((5, 4), -2.0).cuda()
+    g = torch.linspace(0.5, 1.5, 5).cuda()
+    want = token_logprobs(x, ids[:, 0], top_k=3)
+    kw = dict(reduction="none")
+    loss = topk_distillation_loss(x, ids, lp, **kw)
+    leaf = x.clone().requires_grad_()
+    out, row_loss = token_logprobs(leaf, ids[:, 0], top_k=3), topk_distillation_loss(leaf, ids, lp, **kw)
+    gx, = torch.autograd.grad(out.logprob, leaf, g, retain_graph=True)
+    gd, = torch.autograd.grad(row_loss, leaf, g, retain_graph=True)
+    for i in (0, 1):
+        got = token_logprobs(negated(x)[i], ids[:, 0], top_k=3)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(topk_distillation_loss(negated(x)[i], ids, negated(lp)[i], **kw), loss)
+        other = negated(x)[i].detach().requires_grad_()
+        got, = torch.autograd.grad(token_logprobs(other, ids[:, 0]).logprob, other, negated(g)[i])
+        assert torch.equal(got, gx)
+        got, = torch.autograd.grad(topk_distillation_loss(other, ids, lp, **kw), other, negated(g)[i])
+        assert torch.equal(got, gd)
+        got, = torch.autograd.grad(out.logprob, leaf, negated(g)[i], retain_graph=True)
+        assert torch.equal(got, gx)
