@@ -122,7 +122,7 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teac
     * ``tail=True``: what the listed probabilities leave of 1 is one more event, the
       ids not listed, whose student probability is the sum over those ids.
       ``tail=False``: the listed values are normalised among themselves (any
-      ``logits / temperature`` of the teacher will do).
+      ``logits / temperature`` of the teacher will do; a list of -inf alone is NaN).
     * A slot with an id below 0 is not used; an id >= V makes its row NaN; an id
       listed twice counts with both probabilities.
     * ``row_mask`` [...] bool: rows where it is False, and rows without a used slot,

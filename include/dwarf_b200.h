@@ -806,7 +806,7 @@ int dwarf_token_logprobs_bwd(const dwarf_token_logprobs_bwd_args* args, void* st
  * probabilities of k listed ids, and its gradient, in one pass over the
  * student's logits:
  *   tail = 1: p_k = exp(l_k), p_* = max(0, 1 - sum p_k) for the ids not listed
- *   tail = 0: p = softmax of the k values, no rest
+ *   tail = 0: p = softmax of the k values, no rest (values of -inf alone: NaN)
  *   loss = sum_k p_k (log p_k - log q_k) + p_* (log p_* - log q_*)
  * with q = softmax(x / temperature) and q_* its sum over the ids not listed
  * (p_* = 0 when every id is listed). Slots with an id below 0 are not used; an

@@ -122,6 +122,7 @@ def topk_distillation(x, ids, logprobs, *, temperature=1.0, tail=True, row_mask=
     terms = torch.where(some, p * (torch.where(some, l, zero) - torch.where(some, logq.gather(-1, at), zero)), zero)
     rest_term = torch.where(rest > 0, rest * (torch.log(rest.clamp(min=1e-300)) - logq_rest), torch.zeros_like(rest))
     loss = terms.sum(-1) + rest_term.squeeze(-1)
+    loss = torch.where(torch.isnan(p.sum(-1)), torch.full_like(loss, math.nan), loss)  # nothing to normalise
     loss_size = (torch.where(some, p * (l.clamp(min=-1e4).abs() + logq.gather(-1, at).abs()), zero).sum(-1)
                  + rest_term.abs().squeeze(-1) + rest.squeeze(-1) * logq_rest.clamp(min=-1e4).abs().squeeze(-1))
     q = torch.exp(logq)
@@ -137,7 +138,7 @@ def topk_distillation(x, ids, logprobs, *, temperature=1.0, tail=True, row_mask=
     grad = torch.where(dead, torch.zeros_like(grad), grad * up)
     # without a finite logit every q is 0, as its logarithm in token_logprobs says: the loss is inf, the gradient 0
     given = weight.squeeze(-1)
-    nothing = torch.where(given > 0, torch.full_like(given, math.inf), given)
+    nothing = torch.where(given > 0, torch.full_like(given, math.inf), given)  # (NaN stays NaN)
     grad = torch.where(empty.unsqueeze(-1), torch.zeros_like(grad) * weight, grad)
     loss = torch.where(empty, nothing, loss)
     loss = torch.where(keep, loss, torch.zeros_like(loss))

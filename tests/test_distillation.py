@@ -522,3 +522,28 @@ def test_rows_without_a_finite_logit(R, V, k, tail, dtype):
     assert torch.isfinite(grad[good]).all() and not grad[1:3].any()
     if k < V:  # (with every id listed and learnt there may be nothing to learn)
         assert grad[0].any() and grad[R - 1].any()
+
+
+def test_oracle_teacher_without_a_value():
+    x, ids, lp = torch.zeros(1, 4), torch.tensor([[0, 1]]), torch.full((1, 2), -math.inf)
+    loss, grad, _, _ = oracle.topk_distillation(x, ids, lp, tail=False)
+    assert torch.isnan(loss).all() and torch.isnan(grad).all()
+    loss, grad, _, _ = oracle.topk_distillation(x, ids, lp)  # all of the mass is the rest's
+    assert abs(loss.item() - math.log(2)) < 1e-12 and torch.isfinite(grad).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [3, 1000, 40000])
+def test_teacher_without_a_value(V):
+    """A list of -inf alone: all mass is the rest's with a tail, NaN without one; unused slots do not count."""
+    from dwarf_v2_b200.distillation import topk_distillation_loss
+
+    x = logits(4, V, "fp32", V).cuda()
+    ids, lp = torch.arange(2).repeat(4, 1).cuda(), torch.full((4, 2), -1.0).cuda()
+    lp[1] = -math.inf
+    lp[2, 1] = -math.inf
+    ids[2, 0], ids[3, 0] = -1, -1
+    check(x, ids, lp, tail=True)
+    check(x, ids, lp, tail=False)
+    rows = topk_distillation_loss(x, ids, lp, tail=False, reduction="none")
+    assert torch.isnan(rows).tolist() == [False, True, True, False]
