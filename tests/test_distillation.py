@@ -547,3 +547,37 @@ def test_teacher_without_a_value(V):
     check(x, ids, lp, tail=False)
     rows = topk_distillation_loss(x, ids, lp, tail=False, reduction="none")
     assert torch.isnan(rows).tolist() == [False, True, True, False]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("V", [13, 1001, 4097])
+def test_views_of_logits(V, dtype):
+    """Rows of larger tensors, at every offset from the 16-byte boundary: the listed ids' bits, the ends and the
+    gradient's rows go by the row's own start."""
+    from dwarf_v2_b200.distillation import topk_distillation_loss
+
+    g = torch.Generator().manual_seed(V)
+    big = (torch.randn(3, 6, V + 9, generator=g) * 3).to(TYPES[dtype]).cuda()
+    views = [big[:, :-1, :V], big[:, 1:, 9:], big[1, :, 1:V + 1], big[:, 2, 3:V + 3], big.transpose(0, 1)[:, :, 5:V + 5],
+             big[:, ::2, 7:V + 7], big[:1, :1, 2:V + 2], big[0, 0, :V].expand(5, V), big[:, :, ::2]]
+    for view in views:
+        n, lead = view.shape[-1], view.shape[:-1]
+        flat = view.reshape(-1, n)
+        k = min(7, n)
+        ids, lp = teacher(len(flat), n, k, V)
+        ids[0, :3] = torch.tensor([0, n - 1, n // 2]).cuda()[:3]  # the ends
+        up = torch.linspace(0.5, 2.0, len(flat)).cuda()
+        want, grad, size, loss_size = oracle.topk_distillation(flat, ids, lp, upstream=up)
+        loss_tol, grad_tol = tolerances(flat, ids, lp, 1.0, loss_size, grad, size, True)
+        leaf = big.clone().requires_grad_()
+        rows = leaf.as_strided(view.shape, view.stride(), view.storage_offset())
+        loss = topk_distillation_loss(rows, ids.reshape(*lead, k), lp.reshape(*lead, k), reduction="none")
+        close(loss.detach().reshape(-1), want, loss_tol, view.shape)
+        got, = torch.autograd.grad(loss, rows, up.reshape(lead))
+        close(got.reshape(-1, n), grad, grad_tol, view.shape)
+        total = topk_distillation_loss(rows, ids.reshape(*lead, k), lp.reshape(*lead, k), reduction="sum")
+        _, grad, size, _ = oracle.topk_distillation(flat, ids, lp)
+        _, grad_tol = tolerances(flat, ids, lp, 1.0, loss_size, grad, size, True)
+        got, = torch.autograd.grad(total, rows)
+        close(got.reshape(-1, n), grad, grad_tol, view.shape)
