@@ -452,6 +452,7 @@ extern "C" int dwarf_topk_distill(const dwarf_topk_distill_args* args, void* str
   if (a.teacher_ids == nullptr || a.teacher_logprobs == nullptr) return DWARF_ERR_NULL;
   if (a.loss == nullptr && (a.grad == nullptr || a.stats == nullptr)) return DWARF_ERR_NULL;
   if (!aligned16(a.stats)) return DWARF_ERR_ALIGN;
+  if ((st = check_elements(a.grad, a.dtype)) != DWARF_OK) return st;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a.dtype == DWARF_F32) return launch_distill<float>(a, s);
   if (a.dtype == DWARF_BF16) return launch_distill<__nv_bfloat16>(a, s);

@@ -643,6 +643,7 @@ extern "C" int dwarf_token_logprobs_bwd(const dwarf_token_logprobs_bwd_args* arg
   const int64_t rows = a.outer * a.inner;
   if (rows == 0) return DWARF_OK;
   if (a.stats == nullptr || a.entropy == nullptr || a.grad == nullptr) return DWARF_ERR_NULL;
+  if ((st = check_elements(a.grad, a.dtype)) != DWARF_OK) return st;
   if (reinterpret_cast<uintptr_t>(a.stats) & 7) return DWARF_ERR_ALIGN;
   if (a.g_logprob != nullptr && a.targets == nullptr) return DWARF_ERR_NULL;
   if (a.g_top != nullptr && (a.top_ids == nullptr || a.top_k < 1)) return DWARF_ERR_NULL;

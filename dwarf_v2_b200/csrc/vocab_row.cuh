@@ -566,6 +566,11 @@ inline int parts_for(int64_t rows, int vectors) {
 // with 128 threads, 58 with a warp; 16384 rows of 16384: 118 and 98; of 32768: 190 and 201.
 inline bool warp_rows(int64_t rows, int vectors, int most) { return vectors <= most && rows > 18 * kNumSMs; }
 
+// Host check of a pointer to elements of a logit type.
+inline int check_elements(const void* p, int32_t dtype) {
+  return reinterpret_cast<uintptr_t>(p) & (dtype == DWARF_F32 ? 3 : 1) ? DWARF_ERR_ALIGN : DWARF_OK;
+}
+
 // Host checks shared by the entry points: sizes, strides and the scale of a logit tensor.
 inline int check_logits(const void* logits, int32_t dtype, int64_t outer, int64_t inner, int64_t vocab, int64_t so,
                         int64_t si, float inv_temperature) {
@@ -576,9 +581,7 @@ inline int check_logits(const void* logits, int32_t dtype, int64_t outer, int64_
   const float c2 = inv_temperature * kLog2e;
   if (!(c2 > 0.0f) || c2 > 3.0e38f) return DWARF_ERR_VALUE;
   if (outer * inner > 0 && logits == nullptr) return DWARF_ERR_NULL;
-  const uintptr_t mask = dtype == DWARF_F32 ? 3 : 1;
-  if (reinterpret_cast<uintptr_t>(logits) & mask) return DWARF_ERR_ALIGN;
-  return DWARF_OK;
+  return check_elements(logits, dtype);
 }
 
 }  // namespace dwarf

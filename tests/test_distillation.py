@@ -581,3 +581,20 @@ def test_views_of_logits(V, dtype):
         _, grad_tol = tolerances(flat, ids, lp, 1.0, loss_size, grad, size, True)
         got, = torch.autograd.grad(total, rows)
         close(got.reshape(-1, n), grad, grad_tol, view.shape)
+
+
+def test_c_entries_refuse_a_gradient_off_its_elements():
+    import ctypes
+
+    from dwarf_v2_b200 import _lib
+
+    lib = _lib.load()
+    base = dict(version=_lib.ABI_VERSION, logits=4096, outer=1, inner=2, vocab=64, so=0, si=64, inv_temperature=1.0,
+                stats=4096)
+    for dtype, off in ((0, 2), (0, 1), (1, 1), (2, 1)):
+        args = _lib.TokenLogprobsBwdArgs(**base, dtype=dtype, entropy=4096, grad=4096 + off)
+        assert lib.dwarf_token_logprobs_bwd(ctypes.byref(args), None) == -5
+        for loss in (None, 4096):
+            args = _lib.TopkDistillArgs(**base, dtype=dtype, k=4, teacher_ids=4096, teacher_logprobs=4096, loss=loss,
+                                        loss_scale=1.0, scale=1.0, grad=4096 + off)
+            assert lib.dwarf_topk_distill(ctypes.byref(args), None) == -5
