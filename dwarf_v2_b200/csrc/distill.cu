@@ -363,7 +363,9 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
 // is read, under a policy that keeps it there, and the threads of a CTA are chosen so that the
 // rows in flight are about 40 MB. 16384 rows of 32768 bf16, 64 entries: 390 us (128 threads
 // without either: 534, with 475 MB read for 268; the row held in shared memory: 483; 512
-// threads: 540). The loss alone: 128 threads, no prefetch, 199 us (256 threads: 249).
+// threads: 540). It ends at 512 threads: against two passes over the rows at the copy's rate the
+// launch takes 1.28 times as long at 32768 bf16, 1.29 at 131072, and 1.51 at 262144 (fp32: 1.18 at
+// 32768, 1.47 at 131072), where two rows on each SM are 155 MB and the second pass leaves L2. The loss alone: 128 threads, no prefetch, 199 us (256 threads: 249).
 template <typename T, int NT, bool kGrad>
 __global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_kernel(const dwarf_topk_distill_args a, int cluster) {
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;

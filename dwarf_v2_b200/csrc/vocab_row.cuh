@@ -500,7 +500,9 @@ struct Part {
 };
 
 // Where the values of a row's vectors go: whole vectors at once where the output row lies
-// on the same 16-byte boundaries as the logits, else (a slice of an odd vocabulary) by element.
+// on the same 16-byte boundaries as the logits, else (a slice of an odd vocabulary) by element:
+// 8 x 512 rows of logits[:, :-1] at 32003 bf16 take 392 us (log probability and gradient), the same
+// rows contiguous 144.
 template <typename T>
 struct RowStore {
   static constexpr int kVec = Vec16<T>::kVec;

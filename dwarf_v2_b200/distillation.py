@@ -135,8 +135,9 @@ def topk_distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teac
     * ``reduction``: "mean" over the rows that ``row_mask`` keeps, "sum", or "none"
       ([...]). The loss is fp32; no factor temperature**2 is applied.
 
-    Second and forward-mode derivatives and torch.func transforms are refused. Runs on the
-    current stream, without synchronising.
+    The same call gives the same bits every time; a row's last bits may change with the number
+    of rows beside it. Second and forward-mode derivatives and torch.func transforms are
+    refused. Runs on the current stream, without synchronising.
     """
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")

@@ -108,7 +108,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     A row without a finite logit gives logprob, lse and top_logprobs -inf, entropy 0
     and a gradient of zeros; a row with NaN or +inf gives NaN. Every float output is
     differentiable with respect to the logits; a row whose output gradients are all
-    zero gets exact zeros. Second and forward-mode derivatives and torch.func transforms
+    zero gets exact zeros. The same call gives the same bits every time; a row's last bits
+    may change with the number of rows beside it, which decides how many threads share a row.
+    Second and forward-mode derivatives and torch.func transforms
     are refused. Runs on the current stream, without synchronising.
     """
     _rows.refuse_transforms(logits=logits, targets=targets)

@@ -569,7 +569,9 @@ class DwarfForCausalLM(nn.Module):
         """Per-token log probability of ``targets`` [B, T] (or None), entropy, lse and the ``top_k``
         best alternatives at ``temperature`` (see ``logprobs.token_logprobs``), from bf16 logits as
         ``forward`` computes them. The logits are made 1024 rows at a time, so that [B, T, vocab] never
-        exists and each piece is read back from L2. Inference only; its ``top_ids`` and
+        exists and three quarters of each piece are read back from L2 (16 of its 67 MB from memory). For
+        8 x 2048 tokens that takes 769 us after the hidden states (880 with 64 alternatives) of 3.8 ms;
+        1.07 GB of logits at once would take 620 (677). Inference only; its ``top_ids`` and
         ``top_logprobs`` are what ``distillation.topk_distillation_loss`` takes from a teacher."""
         self._check(input_ids, inference_only=True)
         B, T = input_ids.shape
