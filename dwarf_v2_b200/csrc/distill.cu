@@ -365,7 +365,8 @@ __device__ __forceinline__ void distill_row(const dwarf_topk_distill_args& a, in
 // without either: 534, with 475 MB read for 268; the row held in shared memory: 483; 512
 // threads: 540). It ends at 512 threads: against two passes over the rows at the copy's rate the
 // launch takes 1.28 times as long at 32768 bf16, 1.29 at 131072, and 1.51 at 262144 (fp32: 1.18 at
-// 32768, 1.47 at 131072), where two rows on each SM are 155 MB and the second pass leaves L2. The loss alone: 128 threads, no prefetch, 199 us (256 threads: 249).
+// 32768, 1.47 at 131072), where two rows on each SM are 155 MB and the second pass leaves L2.
+// The loss alone: 128 threads, no prefetch, 199 us (256 threads: 249).
 template <typename T, int NT, bool kGrad>
 __global__ void __launch_bounds__(NT, 1024 / NT) topk_distill_kernel(const dwarf_topk_distill_args a, int cluster) {
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
